@@ -490,6 +490,141 @@ int nnz_dispatch_sample(nnz_ctx *ctx, const float *logits, uint32_t count,
 int nnz_dispatch_lm_head_bf16(nnz_ctx *ctx, const void *table, const void *x, float *logits,
                               uint32_t vocab, uint32_t hidden);
 
+/* ---- serving: ragged batches over a paged KV cache -------------------------
+ * New (the reference decodes one sequence over one contiguous cache,
+ * transformer.zig:866-1070): what one step of a server that runs many
+ * sequences calls per layer -- the append, then the attention -- and, on the
+ * logits, the log probabilities.
+ *
+ * A batch holds num_seqs sequences.  Sequence s owns rows q_starts[s] ..
+ * q_starts[s+1] of the token buffers, its new tokens in order, n_s of them
+ * (none is allowed); kv_lens[s] counts its tokens with those n_s.  Row i of it
+ * stands at position kv_lens[s] - n_s + i.  Position j lives in slot
+ * j % page_size of page page_table[s * table_width + j / page_size].  An entry
+ * >= num_pages (NNZ_NO_PAGE, say) names no page: nothing is appended there and
+ * nothing there is attended to.  Rows past q_starts[num_seqs] are left as they
+ * were.
+ *
+ * The three arrays are device memory, read when the kernels run, so that a
+ * captured call serves later steps; the bounds num_rows (rows of the buffers),
+ * max_q_len and max_kv_len are the host's, size the launch and must hold for
+ * what the arrays say then.  What lies beyond them is never touched: rows
+ * beyond num_rows do not exist, of a longer q_len only the first max_q_len rows
+ * are computed, a longer kv_len counts as max_kv_len. */
+#define NNZ_NO_PAGE 0xFFFFFFFFu
+typedef struct {
+    void *k_pages;           /* [num_pages][num_kv_heads][page_size][head_dim] */
+    void *v_pages;           /* [num_pages][num_kv_heads][head_dim][page_size] */
+    uint32_t num_pages;
+    uint32_t page_size;      /* a power of two from 16 to 1024 */
+    uint32_t num_kv_heads;
+    uint32_t head_dim;       /* 64 or 128 */
+    uint32_t dtype;          /* NNZ_F16 or NNZ_BF16, of q, k, v and the outputs too */
+    uint32_t reserved;       /* unused */
+} nnz_paged_kv;
+
+typedef struct {
+    const uint32_t *page_table;  /* device [num_seqs][table_width] */
+    const uint32_t *q_starts;    /* device [num_seqs + 1], not decreasing */
+    const uint32_t *kv_lens;     /* device [num_seqs] */
+    uint32_t num_seqs, table_width;
+    uint32_t num_rows, max_q_len, max_kv_len;   /* max_kv_len <= table_width * page_size */
+    uint32_t reserved;           /* unused */
+} nnz_paged_batch;
+
+/* Per-head RMSNorm and rotation of the batch's new queries and keys, and the
+ * append of k and v to the pages, in one pass (dispatchFusedNormRoPE
+ * transformer.zig:829 and dispatchFusedKNormRoPEKVCache :866 for many tokens).
+ * q [row][num_query_heads][head_dim] -> q_out (may be q itself); k and v
+ * [row][num_kv_heads][head_dim].  The strides are elements between rows,
+ * multiples of 8, so that q, k and v may be parts of one buffer; all buffers
+ * 16-byte aligned.
+ *   q_scale, k_scale  f32 [head_dim] norm weights, or NULL: not normalised;
+ *   rotary_dim        dims 0 .. rotary_dim of a head are rotated, a multiple
+ *                     of 16, at most head_dim, 0 for none;
+ *   rope_halves       0: dims 2k and 2k+1 turn together (the reference's
+ *                     convention), 1: dims k and k + rotary_dim/2;
+ *   inv_freq          device f64 [rotary_dim/2] radians per position, or NULL:
+ *                     rope_theta^(-2k/rotary_dim).
+ * Angles are reduced in 64 bits, so far positions rotate as exactly as near
+ * ones; norm and rotation run in f32 and are rounded once, at the store.
+ * A row at a negative position (kv_lens[s] < n_s) is left out.  Two rows that
+ * stand in the same slot of one page race. */
+typedef struct {
+    const float *q_scale, *k_scale;
+    const double *inv_freq;
+    uint32_t num_query_heads;
+    uint32_t q_stride, k_stride, v_stride, q_out_stride;
+    uint32_t rotary_dim, rope_halves;
+    float rope_theta, eps;
+    uint32_t reserved;           /* unused */
+} nnz_paged_append_params;
+int nnz_dispatch_paged_append(nnz_ctx *ctx, const nnz_paged_kv *kv, const nnz_paged_batch *batch,
+                              const void *q, const void *k, const void *v, void *q_out,
+                              const nnz_paged_append_params *params);
+
+/* Attention of the batch's rows over the pages: a chunk of a prompt, single
+ * tokens, drafts that are checked together, or all of them in one batch.
+ * Row at position p, query head h: x_j = scale * q.k_j over the visible
+ * positions j; softcap > 0 makes it softcap * tanh(x_j / softcap); slopes adds
+ * -slopes[h] * |p - j|; output = sum softmax(x)_j v_j, lse = log sum exp(x_j)
+ * (f32 [row][num_query_heads], or NULL).  j is visible if it is below
+ * kv_lens[s], not after p or else below prefix_lens[s], within the window
+ * (j > p - window), and on a page.  A row that sees nothing, or whose scores
+ * are all -inf, gives zeros and lse -inf.  What masked positions hold,
+ * infinities and NaN included, has no influence.
+ * Scores, softmax and sums are f32; the weights are rounded to the cache's
+ * type for the product with V.
+ * workspace: nnz_paged_attention_workspace_bytes(kv, batch, num_query_heads)
+ * bytes (0 = none needed), 16-byte aligned; its contents do not matter before
+ * or after.  Calls that overlap, captured ones among them, need one each. */
+typedef struct {
+    const float *slopes;          /* device f32 [num_query_heads], or NULL */
+    const uint32_t *prefix_lens;  /* device [num_seqs], or NULL: 0 */
+    uint32_t num_query_heads;     /* a multiple of num_kv_heads */
+    uint32_t q_stride, out_stride;/* elements between rows, multiples of 8 */
+    uint32_t window;              /* 0: no window */
+    float scale;                  /* > 0, or 0: 1 / sqrt(head_dim) */
+    float softcap;                /* > 0, or 0: not capped */
+} nnz_paged_attn_params;
+size_t nnz_paged_attention_workspace_bytes(const nnz_paged_kv *kv, const nnz_paged_batch *batch,
+                                           uint32_t num_query_heads);
+int nnz_dispatch_paged_attention(nnz_ctx *ctx, const nnz_paged_kv *kv,
+                                 const nnz_paged_batch *batch, const void *q, void *output,
+                                 float *lse, void *workspace, size_t workspace_bytes,
+                                 const nnz_paged_attn_params *params);
+
+/* Log probabilities of given tokens (the distribution that nnz_dispatch_sample
+ * draws from before top-k and top-p, for many rows of logits at once).
+ * logits [rows][row_stride] in NNZ_F32, NNZ_F16 or NNZ_BF16, vocab of each row
+ * used, any alignment of the rows; x = logits / temperature.  All outputs are
+ * f32 or u32 on the device and optional but logprobs:
+ *   lse[row]       log sum exp(x)
+ *   logprobs[row]  x[tokens[row]] - lse
+ *   entropy[row]   -sum p log p
+ *   rank[row]      how many ids come before the token in the order (larger
+ *                  logit, then lower id): 0 is the greedy choice
+ *   top_ids, top_logprobs [row][top_n]: the first top_n <= 64 of that order
+ * -inf logits have probability 0.  A row that is all -inf gives lse and log
+ * probabilities -inf, entropy 0.  A row with NaN or +inf gives NaN for all
+ * three and its order still holds, NaN last in it and never in top_ids (places
+ * left over hold 0xFFFFFFFF and NaN).  A token >= vocab gives log probability
+ * -inf and rank vocab.
+ * workspace: nnz_token_logprobs_workspace_bytes bytes (0 = none needed), 16-byte
+ * aligned; its contents do not matter before or after.  Calls that overlap,
+ * captured ones among them, need one each. */
+typedef struct {
+    uint64_t row_stride;          /* elements between rows, >= vocab */
+    uint32_t rows, vocab, top_n, dtype;
+    float temperature;            /* > 0 */
+    uint32_t reserved;            /* unused */
+} nnz_logprobs_dims;
+size_t nnz_token_logprobs_workspace_bytes(uint32_t rows, uint32_t vocab, uint32_t top_n);
+int nnz_dispatch_token_logprobs(nnz_ctx *ctx, const void *logits, const uint32_t *tokens,
+                                float *logprobs, float *lse, float *entropy, uint32_t *rank,
+                                uint32_t *top_ids, float *top_logprobs, void *workspace,
+                                size_t workspace_bytes, const nnz_logprobs_dims *dims);
+
 /* ---- decoder model: forwardDecode / generate (transformer.zig:2389-4135) -- */
 
 typedef struct {

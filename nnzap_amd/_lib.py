@@ -15,6 +15,7 @@ HEADER = HERE.parent / "include" / "nnz.h"
 
 OK, EINVAL, EUNSUPPORTED, EHIP, ENOMEM, ETIMEOUT, ESTATE = 0, -1, -2, -3, -4, -5, -6
 F32, F16, BF16 = 0, 1, 2
+NO_PAGE = 0xFFFFFFFF              # NNZ_NO_PAGE
 GEMM_STORE_F16, GEMM_STORE_F32, GEMM_RESADD, GEMM_SILU_PAIR = 0, 1, 2, 3
 GQA_NOALLOC_MAX_BYTES = 8 << 20   # NNZ_GQA_NOALLOC_MAX_BYTES
 EMBED_Q1, EMBED_BF16, EMBED_Q4 = 0, 1, 2
@@ -97,6 +98,36 @@ class ModelConfig(C.Structure):
                 ("head_dim", u32), ("max_context_length", u32), ("max_prefill_length", u32),
                 ("group_size", u32), ("rope_theta", f32), ("rms_eps", f32),
                 ("embed_kind", u32), ("lm_head_kind", u32), ("quant_format", u32)]
+
+
+class PagedKV(C.Structure):
+    """nnz_paged_kv: a paged KV cache."""
+    _fields_ = [("k_pages", vp), ("v_pages", vp), ("num_pages", u32), ("page_size", u32),
+                ("num_kv_heads", u32), ("head_dim", u32), ("dtype", u32), ("reserved", u32)]
+
+
+class PagedBatchDesc(C.Structure):
+    """nnz_paged_batch: a ragged batch of sequences over a paged cache."""
+    _fields_ = [("page_table", vp), ("q_starts", vp), ("kv_lens", vp), ("num_seqs", u32),
+                ("table_width", u32), ("num_rows", u32), ("max_q_len", u32), ("max_kv_len", u32),
+                ("reserved", u32)]
+
+
+class PagedAppendParams(C.Structure):
+    _fields_ = [("q_scale", vp), ("k_scale", vp), ("inv_freq", vp), ("num_query_heads", u32),
+                ("q_stride", u32), ("k_stride", u32), ("v_stride", u32), ("q_out_stride", u32),
+                ("rotary_dim", u32), ("rope_halves", u32), ("rope_theta", f32), ("eps", f32),
+                ("reserved", u32)]
+
+
+class PagedAttnParams(C.Structure):
+    _fields_ = [("slopes", vp), ("prefix_lens", vp), ("num_query_heads", u32), ("q_stride", u32),
+                ("out_stride", u32), ("window", u32), ("scale", f32), ("softcap", f32)]
+
+
+class LogprobsDims(C.Structure):
+    _fields_ = [("row_stride", C.c_uint64), ("rows", u32), ("vocab", u32), ("top_n", u32),
+                ("dtype", u32), ("temperature", f32), ("reserved", u32)]
 
 
 P = C.POINTER
@@ -187,6 +218,15 @@ PROTOS = {
     "nnz_rng_seed": (C.c_int, [vp, C.c_uint64, vp]),
     "nnz_dispatch_sample": (C.c_int, [vp, vp, u32, vp, vp, vp, sz, vp, vp]),
     "nnz_dispatch_lm_head_bf16": (C.c_int, [vp, vp, vp, vp, u32, u32]),
+    # serving: ragged batches over a paged cache, log probabilities
+    "nnz_dispatch_paged_append": (C.c_int, [vp, P(PagedKV), P(PagedBatchDesc), vp, vp, vp, vp,
+                                            P(PagedAppendParams)]),
+    "nnz_paged_attention_workspace_bytes": (sz, [P(PagedKV), P(PagedBatchDesc), u32]),
+    "nnz_dispatch_paged_attention": (C.c_int, [vp, P(PagedKV), P(PagedBatchDesc), vp, vp, vp, vp,
+                                               sz, P(PagedAttnParams)]),
+    "nnz_token_logprobs_workspace_bytes": (sz, [u32, u32, u32]),
+    "nnz_dispatch_token_logprobs": (C.c_int, [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz,
+                                              P(LogprobsDims)]),
     # model
     "nnz_model_create": (C.c_int, [vp, P(ModelConfig), P(vp)]),
     "nnz_model_destroy": (C.c_int, [vp]),

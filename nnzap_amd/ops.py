@@ -545,6 +545,184 @@ def dispatch_lm_head_bf16(dev, table, x, logits):
     dev.call("nnz_dispatch_lm_head_bf16", _v(table), _v(x), _v(logits), V, H)
 
 
+# ------------------------------------------------- serving: paged KV cache
+def _refuse(cond, name: str, msg: str) -> None:
+    """Pointers carry no shape, so what a tensor says is checked here, with the
+    library's error; values and alignments are the library's own checks."""
+    if cond:
+        raise NnzError(name, L.EINVAL, msg)
+
+
+def _is_rows(kv, t, rows: int, heads: int) -> bool:
+    """[rows, heads, head_dim] of the cache's type on its device, heads and dims
+    contiguous."""
+    return (t.dtype == kv.dtype and t.shape == (rows, heads, kv.head_dim) and t.stride(2) == 1
+            and (heads == 1 or t.stride(1) == kv.head_dim) and t.device == kv.device)
+
+
+def _is_flat(t, shape, types, device) -> bool:
+    """Absent, or contiguous of that shape, one of those types, on that device."""
+    return t is None or (t.shape == shape and str(t.dtype)[6:] in types and t.is_contiguous()
+                         and t.device == device)
+
+
+_INT = ("int32", "uint32")
+
+
+def _stride(t) -> int:
+    """Elements between rows; a single row's stride says nothing."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+
+
+class PagedKVCache:
+    """A paged KV cache over two caller-owned tensors (or new, zeroed ones, from
+    :meth:`empty`): K pages [num_pages, num_kv_heads, page_size, head_dim] and V
+    pages [num_pages, num_kv_heads, head_dim, page_size], f16 or bf16."""
+
+    def __init__(self, dev: Device, k_pages, v_pages):
+        n = "PagedKVCache"
+        _refuse(k_pages.dim() != 4 or v_pages.dim() != 4, n, "pages have four dimensions")
+        num, heads, size, d = k_pages.shape
+        _refuse(v_pages.shape != (num, heads, d, size), n,
+                "V pages are [num_pages, num_kv_heads, head_dim, page_size]")
+        _refuse(k_pages.dtype != v_pages.dtype or str(k_pages.dtype)[6:] not in ("float16", "bfloat16"),
+                n, "pages are both f16 or both bf16")
+        _refuse(not (k_pages.is_contiguous() and v_pages.is_contiguous()), n,
+                "pages must be contiguous")
+        _refuse(k_pages.device != dev.torch_device or v_pages.device != dev.torch_device, n,
+                "pages are not on the context's device")
+        self.k_pages, self.v_pages = k_pages, v_pages
+        self.dtype, self.device = k_pages.dtype, k_pages.device
+        self.num_kv_heads, self.head_dim, self.page_size = heads, d, size
+        self.desc = L.PagedKV(k_pages.data_ptr(), v_pages.data_ptr(), num, size, heads, d,
+                              dtype_code(k_pages), 0)
+        self.ref = C.byref(self.desc)
+
+    @classmethod
+    def empty(cls, dev: Device, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int,
+              dtype=None):
+        torch = _torch()
+        kw = dict(dtype=dtype or torch.float16, device=dev.torch_device)
+        return cls(dev, torch.zeros(num_pages, num_kv_heads, page_size, head_dim, **kw),
+                   torch.zeros(num_pages, num_kv_heads, head_dim, page_size, **kw))
+
+
+class PagedBatch:
+    """A ragged batch over a paged cache: page_table [num_seqs, width], q_starts
+    [num_seqs + 1], kv_lens [num_seqs], int32 on the device (read when the
+    kernels run), and the host's bounds num_rows, max_q_len and max_kv_len."""
+
+    def __init__(self, page_table, q_starts, kv_lens, num_rows: int, max_q_len: int,
+                 max_kv_len: int):
+        n = "PagedBatch"
+        for t in (page_table, q_starts, kv_lens):
+            _refuse(str(t.dtype)[6:] not in _INT, n,
+                    "page_table, q_starts and kv_lens are 32-bit integers")
+            _refuse(t.device != page_table.device, n,
+                    "page_table, q_starts and kv_lens are on one device")
+            _refuse(not t.is_contiguous(), n, "page_table, q_starts and kv_lens must be contiguous")
+        _refuse(page_table.dim() != 2, n, "page_table is [num_seqs, width]")
+        seqs, width = page_table.shape
+        _refuse(q_starts.shape != (seqs + 1,) or kv_lens.shape != (seqs,), n,
+                "q_starts is [num_seqs + 1], kv_lens [num_seqs]")
+        self.page_table, self.q_starts, self.kv_lens = page_table, q_starts, kv_lens
+        self.num_rows, self.num_seqs = num_rows, seqs
+        self.desc = L.PagedBatchDesc(page_table.data_ptr(), q_starts.data_ptr(),
+                                     kv_lens.data_ptr(), seqs, width, num_rows, max_q_len,
+                                     max_kv_len, 0)
+        self.ref = C.byref(self.desc)
+
+
+def dispatch_paged_append(dev, kv: PagedKVCache, batch: PagedBatch, q, k, v, q_out, q_scale=None,
+                          k_scale=None, eps: float = 1e-6, theta: float = 1e6,
+                          rotary_dim: int | None = None, halves: bool = False, inv_freq=None):
+    """Per-head norm (where a scale is given) and rotation of a ragged batch's
+    q [rows, Hq, D] -> q_out and k [rows, Hkv, D], k and v appended to their
+    pages (transformer.zig:829 and :866 for many tokens).  Rows may be strided;
+    rotary_dim defaults to D, inv_freq (f64) to theta^(-2k/rotary_dim)."""
+    n, rows, d, hkv = "nnz_dispatch_paged_append", batch.num_rows, kv.head_dim, kv.num_kv_heads
+    hq = q.shape[1] if q.dim() == 3 else 0
+    _refuse(not (_is_rows(kv, q, rows, hq) and _is_rows(kv, q_out, rows, hq)), n,
+            "q and q_out are [num_rows, heads, head_dim] of the cache's type and device")
+    _refuse(not (_is_rows(kv, k, rows, hkv) and _is_rows(kv, v, rows, hkv)), n,
+            "k and v are [num_rows, num_kv_heads, head_dim] of the cache's type and device")
+    rot = d if rotary_dim is None else rotary_dim
+    _refuse(not (_is_flat(q_scale, (d,), ("float32",), kv.device)
+                 and _is_flat(k_scale, (d,), ("float32",), kv.device)
+                 and _is_flat(inv_freq, (rot // 2,), ("float64",), kv.device)), n,
+            "norm scales are f32 [head_dim], inv_freq f64 [rotary_dim / 2], on the cache's device")
+    _refuse(batch.page_table.device != kv.device, n, "batch and cache are on two devices")
+    p = L.PagedAppendParams(_ptr(q_scale), _ptr(k_scale), _ptr(inv_freq), hq, _stride(q),
+                            _stride(k), _stride(v), _stride(q_out), rot, int(halves), theta, eps,
+                            0)
+    dev.call(n, kv.ref, batch.ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(),
+             C.byref(p))
+
+
+def paged_attention_workspace_bytes(kv: PagedKVCache, batch: PagedBatch,
+                                    num_query_heads: int) -> int:
+    return int(lib().nnz_paged_attention_workspace_bytes(kv.ref, batch.ref, num_query_heads))
+
+
+def dispatch_paged_attention(dev, kv: PagedKVCache, batch: PagedBatch, q, out, workspace,
+                             lse=None, scale: float = 0.0, softcap: float = 0.0, window: int = 0,
+                             slopes=None, prefix_lens=None):
+    """Causal attention of a ragged batch's rows q [rows, Hq, D] over the pages
+    (chunks of prompts and single tokens alike) -> out, and optionally lse f32
+    [rows, Hq].  softcap caps the scores, slopes f32 [Hq] biases them by
+    distance, window and prefix_lens int32 [num_seqs] shape the mask."""
+    n, rows = "nnz_dispatch_paged_attention", batch.num_rows
+    hq = q.shape[1] if q.dim() == 3 else 0
+    _refuse(not (_is_rows(kv, q, rows, hq) and _is_rows(kv, out, rows, hq)), n,
+            "q and out are [num_rows, heads, head_dim] of the cache's type and device")
+    _refuse(not (_is_flat(lse, (rows, hq), ("float32",), kv.device)
+                 and _is_flat(slopes, (hq,), ("float32",), kv.device)
+                 and _is_flat(prefix_lens, (batch.num_seqs,), _INT, kv.device)), n,
+            "lse is f32 [num_rows, heads], slopes f32 [heads], prefix_lens int32 [num_seqs], "
+            "on the cache's device")
+    _refuse(batch.page_table.device != kv.device, n, "batch and cache are on two devices")
+    p = L.PagedAttnParams(_ptr(slopes), _ptr(prefix_lens), hq, _stride(q), _stride(out), window,
+                          scale, softcap)
+    dev.call(n, kv.ref, batch.ref, q.data_ptr(), out.data_ptr(), _ptr(lse), _ptr(workspace),
+             workspace.numel() * workspace.element_size() if workspace is not None else 0,
+             C.byref(p))
+
+
+def token_logprobs_workspace_bytes(rows: int, vocab: int, top_n: int = 0) -> int:
+    return int(lib().nnz_token_logprobs_workspace_bytes(rows, vocab, top_n))
+
+
+def dispatch_token_logprobs(dev, logits, tokens, logprobs, workspace, lse=None, entropy=None,
+                            rank=None, top_ids=None, top_logprobs=None, temperature: float = 1.0):
+    """Log probability of tokens[row] under softmax(logits[row] / temperature),
+    with the row's lse, entropy, the token's rank and the best alternatives (as
+    many as top_ids / top_logprobs have columns).  logits [rows, vocab] f32, f16
+    or bf16, rows may be strided; integers are int32."""
+    n = "nnz_dispatch_token_logprobs"
+    _refuse(logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1), n,
+            "logits are [rows, vocab] with contiguous rows")
+    _refuse(str(logits.dtype)[6:] not in _DT, n, "logits are f32, f16 or bf16")
+    rows, vocab = logits.shape
+    top = next((t.shape[1] for t in (top_ids, top_logprobs) if t is not None and t.dim() == 2), 0)
+    one, table, f, at = (rows,), (rows, top), ("float32",), logits.device
+    _refuse(not (_is_flat(tokens, one, _INT, at) and _is_flat(logprobs, one, f, at)
+                 and _is_flat(lse, one, f, at) and _is_flat(entropy, one, f, at)
+                 and _is_flat(rank, one, _INT, at) and _is_flat(top_ids, table, _INT, at)
+                 and _is_flat(top_logprobs, table, f, at)), n,
+            "tokens, rank and top_ids are int32, the rest f32; [rows] or [rows, top_n], contiguous, "
+            "on the logits' device")
+    _refuse(at != dev.torch_device, n, "logits are not on the context's device")
+    stride = logits.stride(0) if rows > 1 else vocab
+    d = L.LogprobsDims(stride, rows, vocab, top, dtype_code(logits), temperature, 0)
+    dev.call(n, logits.data_ptr(), _ptr(tokens), _ptr(logprobs), _ptr(lse), _ptr(entropy),
+             _ptr(rank), _ptr(top_ids), _ptr(top_logprobs), _ptr(workspace),
+             workspace.numel() * workspace.element_size() if workspace is not None else 0,
+             C.byref(d))
+
+
 __all__ = [n for n in dir() if n.startswith("dispatch_")] + ["Device", "DeviceQWeight",
                                                              "NnzError", "gqa_scratch_bytes",
-                                                             "rng_seed", "sample_workspace_bytes"]
+                                                             "rng_seed", "sample_workspace_bytes",
+                                                             "PagedKVCache", "PagedBatch",
+                                                             "paged_attention_workspace_bytes",
+                                                             "token_logprobs_workspace_bytes"]
