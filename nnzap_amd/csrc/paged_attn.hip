@@ -1,8 +1,47 @@
 // Attention of a ragged batch over a paged KV cache (nnz.h,
-// nnz_dispatch_paged_attention).
+// nnz_dispatch_paged_attention), on the matrix cores.
+//
+// The rows of a sequence and KV head are the pairs (token, query head of the
+// group), row r = token * G + head, so that one pass over K and V serves all G
+// heads, and a single token of G heads is a matrix product too.  Both kernels
+// compute scores transposed, S^T[key][row] = K . Q^T, with K as the A operand
+// in a key order that leaves the accumulators holding, per lane, the eight
+// consecutive keys that the second product O^T[dim][row] += V^T . P^T wants of
+// it as its B operand: the weights never move between lanes.  V's pages are
+// transposed, so V^T's A operand is 16 contiguous bytes of a page.
+//
+//   few_kernel    at most 16 rows (single tokens, drafts): bound by the bytes
+//                 of K and V, which go straight from memory into the operand
+//                 registers, each byte once; keys are split over waves and
+//                 blocks, merge_few_kernel joins the blocks' parts.
+//   chunk_kernel  more rows (chunks of prompts): bound by the matrix cores and
+//                 the softmax's vector work beside them; 128 rows a block, K
+//                 and V tiles of 64 keys in LDS, two buffers.
+//
+// The softmax is the online one in base 2: sums are kept relative to a
+// reference M per row, which follows the row's maximum only when that runs
+// ahead by more than 2^8 (weights up to 2^8 cost no precision: f16 and bf16
+// weights are relative to themselves and the sums are f32), so that most steps
+// rescale nothing.
 #include "paged_dev.h"
 
+#include <algorithm>
+
 namespace {
+
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef float float2v __attribute__((ext_vector_type(2)));
+typedef float float4v __attribute__((ext_vector_type(4)));
+typedef float float16v __attribute__((ext_vector_type(16)));
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf2v __attribute__((ext_vector_type(2)));
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+
+constexpr uint32_t FEW = 16;      // most rows of few_kernel
+constexpr uint32_t TILE_ROWS = 128;
+constexpr uint32_t KT = 64;       // keys per tile of chunk_kernel
+constexpr float LN2 = 0.69314718055994531f, LOG2E = 1.44269504088896341f;
 
 struct AttnArgs {
     PagedView b;
@@ -13,67 +52,716 @@ struct AttnArgs {
     const uint32_t *prefix;
     uint64_t q_stride, o_stride;
     uint32_t hq, G, window;
-    float scale, cap;
+    float scale;          // of the scores, times log2 e
+    float cap_in, cap;    // softcap: cap * tanh(x) with 2 log2(e) x = cap_in * (q . k); cap times log2 e
+    uint32_t few;         // sequences of at most this many rows are few_kernel's
+    uint32_t units;       // row tiles of the whole batch, an upper bound
+    uint32_t splits, chunk;
+    float *part_o, *part_ml;
 };
 
-// One wave per (row, query head): 64 keys a step, lane l scores key l, then
-// owns dims l, l + 64 of the output.
-template <int D, bool BF>
-__global__ __launch_bounds__(64) void attn_kernel(AttnArgs a) {
-    const uint32_t row = blockIdx.x, h = blockIdx.y, l = threadIdx.x, hk = h / a.G;
-    uint32_t s = 0;
-    while (s < a.b.num_seqs && a.b.starts[s + 1] <= row) ++s;
-    if (s == a.b.num_seqs) return;
-    const PagedSeq sq = paged_seq(a.b, s);
-    if (row < sq.row0 || row - sq.row0 >= sq.n || row - sq.row0 >= a.b.max_q) return;
-    const int32_t p = sq.first + (int32_t)(row - sq.row0);
-    const PagedSpan span = paged_span(p, sq.len, a.prefix ? a.prefix[s] : 0u, a.window);
-    __shared__ float q[D];
-    __shared__ float w[64];
-    __shared__ size_t base[64];
-    for (uint32_t d = l; d < D; d += 64) q[d] = paged_load<BF>(a.q[row * a.q_stride + h * D + d]);
-    __syncthreads();
-    float o[D / 64] = {}, m = -INFINITY, sum = 0.f;
-    for (uint32_t j0 = span.lo & ~63u; j0 < span.hi; j0 += 64) {
-        const uint32_t j = j0 + l, slot = j & ((1u << a.b.shift) - 1);
-        const uint32_t page = j >= span.lo && j < span.hi ? paged_page(a.b, s, j) : a.b.num_pages;
-        const bool on = page < a.b.num_pages;
-        const size_t at = ((size_t)page * a.b.hkv + hk) << a.b.shift;
-        float x = -INFINITY;
-        if (on) {
-            const uint16_t *kr = a.k + (at + slot) * D;
-            x = 0.f;
-            for (int d = 0; d < D; ++d) x = fmaf(q[d], paged_load<BF>(kr[d]), x);
-            x *= a.scale;
-            if (a.cap > 0.f) x = a.cap * tanhf(x / a.cap);
-            if (a.slopes) x -= a.slopes[h] * fabsf((float)(p - (int32_t)j));
+template <bool BF>
+__device__ __forceinline__ float4v mfma16(v4u a, v4u b, float4v c) {
+    if constexpr (BF)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, a), __builtin_bit_cast(bf8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
+}
+template <bool BF>
+__device__ __forceinline__ float16v mfma32(v4u a, v4u b, float16v c) {
+    if constexpr (BF)
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf8, a), __builtin_bit_cast(bf8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
+}
+
+// Two values rounded to nearest into one word.
+template <bool BF>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    const float2v f = {a, b};
+    if constexpr (BF) return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, bf2v));
+    else return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, half2v));
+}
+
+// Nonzero if any of the eight values is NaN or infinite.
+template <bool BF>
+__device__ __forceinline__ uint32_t nonfinite(v4u v) {
+    constexpr uint32_t EXP = BF ? 0x7F807F80u : 0x7C007C00u, STEP = BF ? 0x00800080u : 0x04000400u;
+    uint32_t bad = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bad |= (v[i] & EXP) + STEP;
+    return bad & 0x80008000u;
+}
+
+// O^T += V^T . P^T for a V with NaN or infinities, where some rows see only a
+// part of the step: a hidden key's weight of 0 must not meet them, while the
+// rows that do see it get what they should.  The product takes V without them;
+// products of their places (1 each) with the keys' visibility (bit e of vis is
+// this lane's key e) say which sums they belong to.
+template <bool BF, class ACC, class MFMA>
+__device__ __forceinline__ void add_nonfinite(ACC &o, v4u v, v4u p, uint32_t vis, MFMA mfma) {
+    constexpr uint32_t EXP = BF ? 0x7F80u : 0x7C00u, ONE = BF ? 0x3F80u : 0x3C00u;
+    v4u seen = {}, x = {};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const uint32_t sh = 16 * (e & 1), u = v[e >> 1] >> sh & 0xFFFFu;
+        seen[e >> 1] |= (vis >> e & 1 ? ONE : 0u) << sh;
+        x[e >> 1] |= ((u & 0x7FFFu) < EXP ? u : 0u) << sh;
+    }
+    o = mfma(x, p, o);
+    for (int kind = 0; kind < 3; ++kind) {   // NaN, +inf, -inf
+        const uint32_t first = kind == 0 ? EXP + 1 : kind == 1 ? EXP : EXP | 0x8000u;
+        const uint32_t mask = kind == 0 ? 0x7FFFu : 0xFFFFu, last = kind == 0 ? 0x7FFFu : first;
+        const float val = kind == 0 ? __builtin_nanf("") : kind == 1 ? INFINITY : -INFINITY;
+        x = (v4u){0, 0, 0, 0};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const uint32_t sh = 16 * (e & 1), u = (v[e >> 1] >> sh) & mask;
+            x[e >> 1] |= (u >= first && u <= last ? ONE : 0u) << sh;
         }
-        const float mn = fmaxf(m, wave_max(x)), ref = mn == -INFINITY ? 0.f : mn;
-        const float e = expf(x - ref), alpha = expf(m - ref);
-        m = mn;
-        sum = sum * alpha + wave_sum(on ? e : 0.f);
-        __syncthreads();
-        w[l] = on ? e : 0.f;
-        base[l] = on ? at * D + slot : ~(size_t)0;
-        __syncthreads();
-        for (int i = 0; i < D / 64; ++i) {
-            o[i] *= alpha;
-            for (int t = 0; t < 64; ++t)
-                if (base[t] != ~(size_t)0)
-                    o[i] = fmaf(w[t], paged_load<BF>(a.v[base[t] + ((size_t)(l + 64 * i) << a.b.shift)]), o[i]);
+        ACC t = {};
+        t = mfma(x, seen, t);
+#pragma unroll
+        for (int e = 0; e < (int)(sizeof(ACC) / 4); ++e) o[e] += t[e] > 0.f ? val : 0.f;
+    }
+}
+
+// A score as the definition has it, in log2 units (capped scores or a bias);
+// plain scores stay products and are scaled in the exponent.
+__device__ __forceinline__ float general_score(const AttnArgs &a, float s, float slope, int32_t distance) {
+    float t = a.scale * s;
+    if (a.cap > 0.f)   // tanh(x) = 1 - 2 / (e^2x + 1)
+        t = a.cap * fmaf(-2.f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(a.cap_in * s) + 1.f), 1.f);
+    return fmaf(-slope, fabsf((float)distance), t);
+}
+
+// A table entry through the scalar cache (the table does not change while the
+// kernel runs); num_pages where there is no page or the keys are not wanted.
+__device__ __forceinline__ uint32_t page_at(const PagedView &b, uint32_t s, uint32_t key, bool wanted) {
+    const uint32_t e = key >> b.shift;
+    if (!wanted || e >= b.width) return b.num_pages;
+    typedef const uint32_t __attribute__((address_space(4))) *table_t;
+    const table_t t = (table_t)(uintptr_t)(b.table + (size_t)s * b.width);
+    return paged_min(t[e], b.num_pages);
+}
+
+// ---------------------------------------------------------------- few rows
+// A step is 32 keys of a wave: K as two A operands of 16 keys (row m of operand
+// i is key 8 (m >> 2) + 4 i + (m & 3), so lane group g's accumulators hold keys
+// 8 g .. 8 g + 7), V^T as D/16 A operands.  The next step's loads are issued
+// before the current one is computed.  Block = 4 waves that take the steps of
+// a chunk in turn.
+template <int D, bool BF>
+struct FewStep {
+    v4u k[2][D / 32], v[D / 16];
+    uint32_t bad;   // groups of 16 keys without a page
+};
+
+template <int D, bool BF, bool GEN>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void few_kernel(AttnArgs a) {
+    constexpr int NKS = D / 32, NDT = D / 16;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane >> 4, c = lane & 15;
+    const uint32_t hkv = a.b.hkv, kvh = blockIdx.x % hkv, z = blockIdx.x / hkv % a.splits,
+                   s = blockIdx.x / hkv / a.splits;
+    const PagedSeq sq = paged_seq(a.b, s);
+    const uint32_t n = paged_min(sq.n, a.b.max_q), R = n * a.G;
+    if (R == 0 || R > FEW) return;
+    const uint32_t prefix = a.prefix ? a.prefix[s] : 0u;
+    const PagedSpan sp0 = paged_span(sq.first, sq.len, prefix, a.window);
+    const PagedSpan sp1 = paged_span(sq.first + (int32_t)n - 1, sq.len, prefix, a.window);
+    const uint32_t lo = sp0.lo & ~31u, hi = sp1.hi, steps = hi > lo ? (hi - lo + 31) / 32 : 0;
+    const uint32_t nz = steps > a.chunk ? (steps + a.chunk - 1) / a.chunk : 1;
+    if (z >= nz) return;
+    const uint32_t st1 = paged_min(steps, (z + 1) * a.chunk);
+
+    const uint32_t r = paged_min((uint32_t)c, R - 1), tok = r / a.G, head = kvh * a.G + r % a.G;
+    const int32_t pos = sq.first + (int32_t)tok;
+    const PagedSpan sp = paged_span(pos, sq.len, prefix, a.window);
+    const float slope = GEN && a.slopes ? a.slopes[head] * LOG2E : 0.f;
+    v4u qf[NKS];
+    {
+        const uint16_t *qp = a.q + (sq.row0 + tok) * a.q_stride + head * D;
+#pragma unroll
+        for (int ks = 0; ks < NKS; ++ks) qf[ks] = *(const v4u *)(qp + 32 * ks + 8 * g);
+    }
+
+    const uint32_t pmask = (1u << a.b.shift) - 1;
+    auto load = [&](FewStep<D, BF> &f, uint32_t st) __attribute__((always_inline)) {
+        const uint32_t k0 = lo + 32 * st;
+        uint32_t pa = page_at(a.b, s, k0, true), pb = page_at(a.b, s, k0 + 16, k0 + 16 < hi);
+        f.bad = (pa == a.b.num_pages ? 1u : 0u) | (pb == a.b.num_pages ? 2u : 0u);
+        pa = f.bad & 1 ? 0u : pa;   // any page: the keys are masked
+        pb = f.bad & 2 ? 0u : pb;
+        const size_t ha = (size_t)pa * hkv + kvh, hb = (size_t)pb * hkv + kvh;
+        const uint32_t oa = k0 & pmask, ob = (k0 + 16) & pmask;
+        const uint16_t *ka = a.k + ((ha << a.b.shift) + oa) * D, *kb = a.k + ((hb << a.b.shift) + ob) * D;
+        const uint16_t *kp = (c < 8 ? ka : kb) + (8 * (c >> 2 & 1) + (c & 3)) * D + 8 * g;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int ks = 0; ks < NKS; ++ks) f.k[i][ks] = *(const v4u *)(kp + 4 * i * D + 32 * ks);
+        const uint16_t *va = a.v + ((ha * D) << a.b.shift) + oa, *vb = a.v + ((hb * D) << a.b.shift) + ob;
+        const uint16_t *vp = (g < 2 ? va : vb) + ((size_t)c << a.b.shift) + 8 * (g & 1);
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) f.v[dt] = *(const v4u *)(vp + ((size_t)(16 * dt) << a.b.shift));
+    };
+
+    float4v o[NDT];
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) o[dt] = (float4v){0.f, 0.f, 0.f, 0.f};
+    const float cs = GEN ? 1.f : a.scale, ahead = 8.f / cs;
+    float m = -INFINITY, nm = 0.f, l = 0.f;   // reference score, minus it in log2 units, sum of this lane's weights
+    auto compute = [&](const FewStep<D, BF> &f, uint32_t st) __attribute__((always_inline)) {
+        const uint32_t k0 = lo + 32 * st;
+        float sc[8];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float4v t = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int ks = 0; ks < NKS; ++ks) t = mfma16<BF>(f.k[i][ks], qf[ks], t);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[4 * i + e] = t[e];
+        }
+        const uint32_t key = k0 + 8 * g;
+        if constexpr (GEN) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sc[e] = general_score(a, sc[e], slope, pos - (int32_t)(key + e));
+        }
+        const bool masked = k0 < sp1.lo || k0 + 32 > sp0.hi || f.bad;   // wave-uniform
+        uint32_t vis = 0xFF;
+        if (masked) {
+            const bool on = !(f.bad >> (g >> 1) & 1);
+            vis = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) vis |= (on && key + e >= sp.lo && key + e < sp.hi ? 1u : 0u) << e;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sc[e] = vis >> e & 1 ? sc[e] : -INFINITY;
+        }
+        float mx = sc[0];
+#pragma unroll
+        for (int e = 1; e < 8; ++e) mx = fmaxf(mx, sc[e]);
+        if (__builtin_amdgcn_ballot_w64(mx > m + ahead)) {   // wave-uniform
+            mx = fmaxf(mx, __shfl_xor(mx, 16));
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            const bool move = mx > m + ahead;
+            const float nm2 = move ? -mx * cs : nm;
+            const float alpha = move && m != -INFINITY ? __builtin_amdgcn_exp2f(nm2 - nm) : 1.f;
+            m = move ? mx : m;
+            nm = nm2;
+            l *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt) o[dt] *= alpha;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            sc[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], cs, nm));
+            l += sc[e];
+        }
+        v4u p;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = pack2<BF>(sc[2 * i], sc[2 * i + 1]);
+        if (masked) {
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt) {
+                if (__builtin_amdgcn_ballot_w64(nonfinite<BF>(f.v[dt]) != 0))   // wave-uniform, rare
+                    add_nonfinite<BF>(o[dt], f.v[dt], p, vis, mfma16<BF>);
+                else
+                    o[dt] = mfma16<BF>(f.v[dt], p, o[dt]);
+            }
+        } else {
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt) o[dt] = mfma16<BF>(f.v[dt], p, o[dt]);
+        }
+    };
+
+    uint32_t st = z * a.chunk + (uint32_t)w;
+    if (st < st1) {   // wave-uniform, all of it
+        FewStep<D, BF> f0, f1;
+        load(f0, st);
+        for (;;) {
+            if (st + 4 < st1) load(f1, st + 4);
+            compute(f0, st);
+            st += 4;
+            if (st >= st1) break;
+            if (st + 4 < st1) load(f0, st + 4);
+            compute(f1, st);
+            st += 4;
+            if (st >= st1) break;
         }
     }
-    const bool none = m == -INFINITY && !(sum != sum);
-    for (int i = 0; i < D / 64; ++i)
-        a.out[row * a.o_stride + h * D + l + 64 * i] = paged_round<BF>(none ? 0.f : o[i] / sum);
-    if (a.lse && l == 0) a.lse[(size_t)row * a.hq + h] = none ? -INFINITY : m + logf(sum);
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+
+    // the four waves' parts, relative to the largest reference
+    __shared__ float4v so[4][NDT][64];
+    __shared__ float sm[4][16], sl[4][16];
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) so[w][dt][lane] = o[dt];
+    if (g == 0) {
+        sm[w][c] = m == -INFINITY ? -INFINITY : -nm;
+        sl[w][c] = l;
+    }
+    __syncthreads();
+    float M = sm[0][c], wt[4];
+#pragma unroll
+    for (int i = 1; i < 4; ++i) M = fmaxf(M, sm[i][c]);
+    l = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        wt[i] = sm[i][c] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sm[i][c] - M);
+        l += wt[i] * sl[i][c];
+        if (sl[i][c] != sl[i][c]) l = sl[i][c];
+    }
+    const bool mine = (uint32_t)c < R;
+    if (nz == 1) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        uint16_t *op = a.out + (sq.row0 + tok) * a.o_stride + head * D + 4 * g;
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) {
+            if (dt % 4 != w) continue;
+            float4v t = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (wt[i] != 0.f) t += so[i][dt][lane] * wt[i];
+            if (l != l) t = (float4v){l, l, l, l};
+            if (mine)
+                *(uint2 *)(op + 16 * dt) = make_uint2(pack2<BF>(t[0] * inv, t[1] * inv), pack2<BF>(t[2] * inv, t[3] * inv));
+        }
+        if (a.lse && mine && g == 0 && w == 0)
+            a.lse[(size_t)(sq.row0 + tok) * a.hq + head] = l == 0.f ? -INFINITY : (M + __builtin_amdgcn_logf(l)) * LN2;
+        return;
+    }
+    const size_t part = (((size_t)s * hkv + kvh) * a.splits + z) * FEW + (uint32_t)c;
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) {
+        if (dt % 4 != w) continue;
+        float4v t = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (wt[i] != 0.f) t += so[i][dt][lane] * wt[i];
+        if (mine) *(float4v *)(a.part_o + part * D + 16 * dt + 4 * g) = t;
+    }
+    if (mine && g == 0 && w == 0) {
+        a.part_ml[2 * part] = M;
+        a.part_ml[2 * part + 1] = l;
+    }
+}
+
+// One row's parts joined by a wave: nz parts, `step` parts apart.
+template <int D, bool BF>
+__device__ __forceinline__ void join_parts(const float *po, const float *ml, size_t first, size_t step, uint32_t nz,
+                                           uint16_t *out, float *lse) {
+    constexpr int V = D / 64;
+    const int lane = threadIdx.x & 63;
+    float M = -INFINITY;
+    for (uint32_t z = lane; z < nz; z += 64) M = fmaxf(M, ml[2 * (first + z * step)]);
+    M = wave_max(M);
+    float l = 0.f, o[V] = {};
+    for (uint32_t z = 0; z < nz; ++z) {
+        const size_t p = first + z * step;
+        const float mz = ml[2 * p], lz = ml[2 * p + 1];
+        const float wt = mz == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mz - M);
+        if (lz != lz) l = lz;
+        if (wt == 0.f) continue;
+        l += wt * lz;
+#pragma unroll
+        for (int i = 0; i < V; ++i) o[i] = fmaf(wt, po[p * D + V * lane + i], o[i]);
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    if constexpr (V == 2) {
+        *(uint32_t *)(out + 2 * lane) = l != l ? pack2<BF>(l, l) : pack2<BF>(o[0] * inv, o[1] * inv);
+    } else {
+        out[lane] = (uint16_t)(l != l ? pack2<BF>(l, l) : pack2<BF>(o[0] * inv, 0.f));
+    }
+    if (lse && lane == 0) *lse = l == 0.f ? -INFINITY : (M + __builtin_amdgcn_logf(l)) * LN2;
+}
+
+// Block = (sequence, KV head), its waves take the rows in turn.
+template <int D, bool BF>
+__global__ __launch_bounds__(256) void merge_few_kernel(AttnArgs a) {
+    const uint32_t hkv = a.b.hkv, kvh = blockIdx.x % hkv, s = blockIdx.x / hkv;
+    const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const PagedSeq sq = paged_seq(a.b, s);
+    const uint32_t n = paged_min(sq.n, a.b.max_q), R = n * a.G;
+    if (R == 0 || R > FEW) return;
+    const uint32_t prefix = a.prefix ? a.prefix[s] : 0u;
+    const uint32_t lo = paged_span(sq.first, sq.len, prefix, a.window).lo & ~31u;
+    const uint32_t hi = paged_span(sq.first + (int32_t)n - 1, sq.len, prefix, a.window).hi;
+    const uint32_t steps = hi > lo ? (hi - lo + 31) / 32 : 0;
+    if (steps <= a.chunk) return;
+    const uint32_t nz = (steps + a.chunk - 1) / a.chunk;
+    for (uint32_t r = w; r < R; r += 4) {
+        const size_t row = sq.row0 + r / a.G;
+        const uint32_t head = kvh * a.G + r % a.G;
+        join_parts<D, BF>(a.part_o, a.part_ml, (((size_t)s * hkv + kvh) * a.splits) * FEW + r, FEW, nz,
+                          a.out + row * a.o_stride + head * D, a.lse ? a.lse + row * a.hq + head : nullptr);
+    }
+}
+
+// ------------------------------------------------------------ chunks of rows
+// 16 bytes per lane from memory straight into LDS: lane i's to lds + 16 i.
+__device__ __forceinline__ void load_to_lds(const void *sbase, uint32_t voff, uint32_t lds) {
+    // five wait states between a VALU write of an SGPR and its use as address
+    asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(sbase), "{m0}"(lds) : "memory");
+}
+
+// What unit u of the batch's row tiles is: tile `tile` of sequence `s`.
+__device__ __forceinline__ bool find_tile(const AttnArgs &a, uint32_t u, uint32_t *s, uint32_t *tile) {
+    const uint32_t lane = threadIdx.x & 63;
+    uint32_t before = 0;
+    for (uint32_t base = 0; base < a.b.num_seqs; base += 64) {
+        uint32_t cnt = 0;
+        if (base + lane < a.b.num_seqs) {
+            const uint32_t rows = paged_min(paged_seq(a.b, base + lane).n, a.b.max_q) * a.G;
+            cnt = rows <= a.few ? 0u : (rows + TILE_ROWS - 1) / TILE_ROWS;
+        }
+        uint32_t upto = cnt;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t t = __shfl_up(upto, o);
+            upto += lane >= (uint32_t)o ? t : 0u;
+        }
+        const uint32_t all = __builtin_amdgcn_readlane(upto, 63);
+        if (u - before < all) {
+            const uint64_t in = __builtin_amdgcn_ballot_w64(u - before < upto);
+            const uint32_t i = __builtin_amdgcn_readfirstlane(__builtin_ctzll(in));
+            *s = base + i;
+            *tile = u - before - __builtin_amdgcn_readlane(upto - cnt, i);
+            return true;
+        }
+        before += all;
+    }
+    return false;
+}
+
+// Tile `tile` of sequence s: its rows and its keys, in tiles of KT.
+struct RowTile {
+    PagedSeq sq;
+    uint32_t R, r0, prefix, lo, hi, t0, t1, nz;
+};
+__device__ __forceinline__ RowTile row_tile(const AttnArgs &a, uint32_t s, uint32_t tile) {
+    RowTile t;
+    t.sq = paged_seq(a.b, s);
+    t.R = paged_min(t.sq.n, a.b.max_q) * a.G;
+    t.r0 = tile * TILE_ROWS;
+    t.prefix = a.prefix ? a.prefix[s] : 0u;
+    const uint32_t last = paged_min(t.r0 + TILE_ROWS, t.R) - 1;
+    t.lo = paged_span(t.sq.first + (int32_t)(t.r0 / a.G), t.sq.len, t.prefix, a.window).lo;
+    t.hi = paged_span(t.sq.first + (int32_t)(last / a.G), t.sq.len, t.prefix, a.window).hi;
+    t.t0 = t.lo / KT;
+    t.t1 = t.hi > t.lo ? (t.hi + KT - 1) / KT : t.t0;
+    t.nz = a.splits > 1 && t.t1 - t.t0 > a.chunk ? (t.t1 - t.t0 + a.chunk - 1) / a.chunk : 1;
+    return t;
+}
+
+// A block owns 128 rows of one KV head, a wave 32 of them
+// (v_mfma_f32_32x32x16); accumulator register 4 j + e of lane half hh is row
+// 8 j + 4 hh + e of a 32-key A operand, whose row m is key m with bits 2 and 3
+// swapped: registers 8 i .. 8 i + 7 are keys 16 i + 8 hh ...  K rows lie in
+// LDS with their 16-byte pieces rotated (piece p of row r at slot p ^ r), V as
+// its pages have it, [16-key group][dim][16 keys], where a wave's operand is
+// one contiguous run.
+template <int D, bool BF, bool GEN>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void chunk_kernel(AttnArgs a) {
+    constexpr int NKS = D / 16, NDT = D / 32, PIECES = D / 8;   // pieces of 16 bytes in a K row
+    constexpr int TILE = KT * D, LOADS = TILE / 8 / 256;
+    __shared__ __align__(16) uint16_t Ks[2][TILE], Vs[2][TILE];
+    const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5, c = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // KV head fastest: with 8 of them each XCD keeps one head's K and V in its L2;
+    // the last tiles, which see the most keys, first
+    const uint32_t hkv = a.b.hkv, kvh = blockIdx.x % hkv, z = blockIdx.x / hkv % a.splits;
+    const uint32_t u = a.units - 1 - blockIdx.x / hkv / a.splits;
+    uint32_t s, tile;
+    if (!find_tile(a, u, &s, &tile)) return;
+    const RowTile rt = row_tile(a, s, tile);
+    if (z >= rt.nz) return;
+    const uint32_t t0 = a.splits > 1 ? rt.t0 + z * a.chunk : rt.t0;
+    const uint32_t t1 = a.splits > 1 ? paged_min(rt.t1, t0 + a.chunk) : rt.t1;
+
+    const uint32_t w0 = rt.r0 + 32u * (uint32_t)wave;
+    const bool any = w0 < rt.R;   // wave-uniform
+    const uint32_t wl = paged_min(w0 + 31, rt.R - 1), r = paged_min(w0 + (uint32_t)c, rt.R - 1);
+    auto span_of = [&](uint32_t row) {
+        return paged_span(rt.sq.first + (int32_t)(row / a.G), rt.sq.len, rt.prefix, a.window);
+    };
+    const PagedSpan first = span_of(paged_min(w0, rt.R - 1)), last = span_of(wl), sp = span_of(r);
+    const uint32_t tok = r / a.G, head = kvh * a.G + r % a.G;
+    const int32_t pos = rt.sq.first + (int32_t)tok;
+    const float slope = GEN && a.slopes ? a.slopes[head] * LOG2E : 0.f;
+
+    // Piece i of this thread: 16 bytes of K row krow(i), of V's group the same;
+    // a wave's pieces lie in one group of 16 keys, hence in one page.
+    constexpr int RPW = 64 / PIECES;   // K rows of a wave's piece
+    const uint32_t krow = (uint32_t)lane / PIECES + (uint32_t)wave * RPW;
+    const uint32_t koff = ((krow & 15) * D + 8 * (((uint32_t)lane % PIECES) ^ (krow & (PIECES - 1)))) * 2u;
+    const uint32_t vp = ((uint32_t)tid) % (2 * D), voff = ((vp / 2) << a.b.shift) * 2u + (vp & 1) * 16u;
+    const uint32_t pmask = (1u << a.b.shift) - 1;
+    struct Pages {
+        uint32_t p[4];
+    };
+    auto pages_of = [&](uint32_t t) __attribute__((always_inline)) {
+        Pages p;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p.p[i] = page_at(a.b, s, t * KT + 16 * i, t < t1 && t * KT + 16 * i < rt.hi);
+        return p;
+    };
+    auto stage = [&](uint32_t t, const Pages &p) __attribute__((always_inline)) {
+        const uint32_t k0 = t * KT, buf = t & 1;
+        const uint32_t lk = __builtin_amdgcn_readfirstlane(
+            (uint32_t)(size_t)(__attribute__((address_space(3))) uint16_t *)(Ks[buf] + 8 * 64 * wave));
+        const uint32_t lv = __builtin_amdgcn_readfirstlane(
+            (uint32_t)(size_t)(__attribute__((address_space(3))) uint16_t *)(Vs[buf] + 8 * 64 * wave));
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            uint32_t page, in;
+            if constexpr (D == 128) {
+                page = p.p[i];
+                in = 16 * i;
+            } else {   // a piece index spans two groups
+                page = wave < 2 ? p.p[2 * i] : p.p[2 * i + 1];
+                in = 32 * i + (wave < 2 ? 0 : 16);
+            }
+            page = page == a.b.num_pages ? 0u : page;   // any page: the keys are masked
+            const size_t h = (size_t)page * hkv + kvh;
+            const uint32_t slot = (k0 + in) & pmask;
+            load_to_lds(a.k + ((h << a.b.shift) + slot) * D, koff, lk + 16u * (uint32_t)(i * 256));
+            load_to_lds(a.v + ((h * D) << a.b.shift) + slot, voff, lv + 16u * (uint32_t)(i * 256));
+        }
+    };
+    auto bad_of = [&](const Pages &p) __attribute__((always_inline)) {
+        uint32_t bad = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bad |= (p.p[i] == a.b.num_pages ? 1u : 0u) << i;
+        return bad;
+    };
+
+    Pages cur{}, next{};
+    if (t0 < t1) {
+        cur = pages_of(t0);
+        stage(t0, cur);
+        next = pages_of(t0 + 1);
+    }
+    v4u qf[NKS];
+    {
+        const uint16_t *qp = a.q + (rt.sq.row0 + tok) * a.q_stride + head * D;
+#pragma unroll
+        for (int ks = 0; ks < NKS; ++ks) qf[ks] = *(const v4u *)(qp + 16 * ks + 8 * hh);
+    }
+    float16v o[NDT];
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[dt][e] = 0.f;
+    const float cs = GEN ? 1.f : a.scale, ahead = 8.f / cs;
+    float m = -INFINITY, nm = 0.f, l = 0.f;
+    const int krm = (c & 19) | ((c & 4) << 1) | ((c & 8) >> 1);   // key of A row c
+
+    for (uint32_t t = t0; t < t1; ++t) {
+        // this tile's loads have arrived, everybody's, and nobody reads the
+        // other buffer any more
+        __builtin_amdgcn_s_waitcnt(7 << 4);   // vmcnt 0, lgkmcnt 0
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        const uint32_t bad = bad_of(cur);
+        if (t + 1 < t1) {   // block-uniform
+            stage(t + 1, next);
+            cur = next;
+            next = pages_of(t + 2);
+        }
+        const uint16_t *const Kt = Ks[t & 1], *const Vt = Vs[t & 1];
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+            const uint32_t kk0 = t * KT + 32u * kt;
+            if (!any || kk0 >= last.hi || kk0 + 32 <= first.lo) continue;   // wave-uniform
+            const int row = 32 * kt + krm;
+            float16v sc;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) sc[e] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < NKS; ++ks) {
+                const v4u kf = *(const v4u *)(Kt + row * D + 8 * ((2 * ks + hh) ^ (row & (PIECES - 1))));
+                sc = mfma32<BF>(kf, qf[ks], sc);
+            }
+            const uint32_t key = kk0 + 8 * hh;   // register e: key + 16 (e >> 3) + (e & 7)
+            if constexpr (GEN) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    sc[e] = general_score(a, sc[e], slope, pos - (int32_t)(key + 16 * (e >> 3) + (e & 7)));
+            }
+            const uint32_t gone = bad >> (2 * kt) & 3;
+            const bool masked = kk0 < last.lo || kk0 + 32 > first.hi || gone;   // wave-uniform
+            uint32_t vis = 0xFFFF;
+            if (masked) {
+                vis = 0;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const uint32_t j = key + 16 * (e >> 3) + (e & 7);
+                    const bool on = j >= sp.lo && j < sp.hi && !(gone >> (e >> 3) & 1);
+                    vis |= (on ? 1u : 0u) << e;
+                    sc[e] = on ? sc[e] : -INFINITY;
+                }
+            }
+            float mx = sc[0];
+#pragma unroll
+            for (int e = 1; e < 16; ++e) mx = fmaxf(mx, sc[e]);
+            if (__builtin_amdgcn_ballot_w64(mx > m + ahead)) {   // wave-uniform
+                const float2 both = swap32(mx, mx);
+                mx = fmaxf(both.x, both.y);
+                const bool move = mx > m + ahead;
+                const float nm2 = move ? -mx * cs : nm;
+                const float alpha = move && m != -INFINITY ? __builtin_amdgcn_exp2f(nm2 - nm) : 1.f;
+                m = move ? mx : m;
+                nm = nm2;
+                l *= alpha;
+#pragma unroll
+                for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o[dt][e] *= alpha;
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                sc[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], cs, nm));
+                l += sc[e];
+            }
+#pragma unroll
+            for (int st = 0; st < 2; ++st) {   // 16 keys each
+                v4u p;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) p[i] = pack2<BF>(sc[8 * st + 2 * i], sc[8 * st + 2 * i + 1]);
+                const uint16_t *const vrow = Vt + (2 * kt + st) * (16 * D) + c * 16 + 8 * hh;
+                if (masked) {
+#pragma unroll
+                    for (int dt = 0; dt < NDT; ++dt) {
+                        const v4u v = *(const v4u *)(vrow + 32 * 16 * dt);
+                        if (__builtin_amdgcn_ballot_w64(nonfinite<BF>(v) != 0))   // wave-uniform, rare
+                            add_nonfinite<BF>(o[dt], v, p, vis >> (8 * st), mfma32<BF>);
+                        else
+                            o[dt] = mfma32<BF>(v, p, o[dt]);
+                    }
+                } else {
+#pragma unroll
+                    for (int dt = 0; dt < NDT; ++dt) o[dt] = mfma32<BF>(*(const v4u *)(vrow + 32 * 16 * dt), p, o[dt]);
+                }
+            }
+        }
+    }
+    const float2 lp = swap32(l, l);
+    l = lp.x + lp.y;
+    if (!any || w0 + (uint32_t)c >= rt.R) return;
+    const float M = -nm;
+    if (rt.nz > 1) {
+        const size_t part = (((size_t)u * hkv + kvh) * a.splits + z) * TILE_ROWS + (w0 - rt.r0) + (uint32_t)c;
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                *(float4v *)(a.part_o + part * D + 32 * dt + 8 * j + 4 * hh) =
+                    (float4v){o[dt][4 * j], o[dt][4 * j + 1], o[dt][4 * j + 2], o[dt][4 * j + 3]};
+        if (hh == 0) {
+            a.part_ml[2 * part] = m == -INFINITY ? -INFINITY : M;
+            a.part_ml[2 * part + 1] = l;
+        }
+        return;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    uint16_t *const op = a.out + (rt.sq.row0 + tok) * a.o_stride + head * D;
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            *(uint2 *)(op + 32 * dt + 8 * j + 4 * hh) =
+                make_uint2(pack2<BF>(o[dt][4 * j] * inv, o[dt][4 * j + 1] * inv),
+                           pack2<BF>(o[dt][4 * j + 2] * inv, o[dt][4 * j + 3] * inv));
+    if (a.lse && hh == 0)
+        a.lse[(size_t)(rt.sq.row0 + tok) * a.hq + head] = l == 0.f ? -INFINITY : (M + __builtin_amdgcn_logf(l)) * LN2;
+}
+
+// Block = 16 rows of a row tile whose keys were split, its waves in turn.
+template <int D, bool BF>
+__global__ __launch_bounds__(256) void merge_chunk_kernel(AttnArgs a) {
+    const uint32_t hkv = a.b.hkv, kvh = blockIdx.x % hkv, u = blockIdx.x / hkv;
+    const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    uint32_t s, tile;
+    if (!find_tile(a, u, &s, &tile)) return;
+    const RowTile rt = row_tile(a, s, tile);
+    if (rt.nz == 1) return;
+    for (uint32_t i = w; i < 16; i += 4) {
+        const uint32_t r = blockIdx.y * 16 + i;
+        if (rt.r0 + r >= rt.R) return;
+        const size_t row = rt.sq.row0 + (rt.r0 + r) / a.G;
+        const uint32_t head = kvh * a.G + (rt.r0 + r) % a.G;
+        join_parts<D, BF>(a.part_o, a.part_ml, ((size_t)u * hkv + kvh) * a.splits * TILE_ROWS + r, TILE_ROWS, rt.nz,
+                          a.out + row * a.o_stride + head * D, a.lse ? a.lse + row * a.hq + head : nullptr);
+    }
+}
+
+// ------------------------------------------------------------------- launch
+// Which kernels run and how keys are split, from the host's bounds alone.
+struct Plan {
+    uint32_t few_splits = 0, few_chunk = 0;                // 0 splits: not launched
+    uint32_t units = 0, chunk_splits = 0, chunk_tiles = 0;
+    size_t few_parts = 0, chunk_parts = 0;                 // rows of partial results
+};
+
+Plan plan_of(const nnz_paged_kv &kv, const nnz_paged_batch &b, uint32_t hq) {
+    Plan p;
+    const uint32_t G = hq / kv.num_kv_heads, hkv = kv.num_kv_heads;
+    const uint64_t most = (uint64_t)b.max_q_len * G;   // rows of a sequence
+    // One sequence whose bound passes 16 rows goes to the chunk kernel, whatever
+    // its length turns out to be; a batch of several may hold both kinds.
+    if (G <= FEW && (most <= FEW || b.num_seqs > 1)) {
+        const uint32_t steps = (b.max_kv_len + 31) / 32, blocks = b.num_seqs * hkv;
+        const uint32_t want = std::max(1u, 2048 / blocks), most_splits = std::max(1u, steps / 16);
+        const uint32_t splits = std::min(want, most_splits);
+        p.few_chunk = (steps + splits - 1) / splits;
+        p.few_splits = (steps + p.few_chunk - 1) / p.few_chunk;
+        if (p.few_splits > 1) p.few_parts = (size_t)blocks * p.few_splits * FEW;
+    }
+    if (most > FEW || G > FEW) {
+        const uint64_t by_rows = (uint64_t)b.num_rows * G / TILE_ROWS + b.num_seqs;
+        const uint64_t by_seqs = (uint64_t)b.num_seqs * ((most + TILE_ROWS - 1) / TILE_ROWS);
+        p.units = (uint32_t)std::min(by_rows, by_seqs);
+        const uint32_t tiles = (b.max_kv_len + KT - 1) / KT;
+        const uint32_t want = std::max(1u, 512 / (p.units * hkv)), most_splits = std::max(1u, tiles / 4);
+        const uint32_t splits = std::min(want, most_splits);
+        p.chunk_tiles = (tiles + splits - 1) / splits;
+        p.chunk_splits = (tiles + p.chunk_tiles - 1) / p.chunk_tiles;
+        if (p.chunk_splits > 1) p.chunk_parts = (size_t)p.units * hkv * p.chunk_splits * TILE_ROWS;
+    }
+    return p;
+}
+
+size_t bytes_of(const Plan &p, uint32_t head_dim) { return (p.few_parts + p.chunk_parts) * (head_dim + 2) * 4; }
+
+template <int D, bool BF, bool GEN>
+void start(hipStream_t stream, const Plan &p, AttnArgs a, float *ws) {
+    const uint32_t hkv = a.b.hkv;
+    if (p.chunk_splits) {
+        a.units = p.units;
+        a.splits = p.chunk_splits;
+        a.chunk = p.chunk_tiles;
+        a.part_o = ws;
+        a.part_ml = ws + p.chunk_parts * D;
+        chunk_kernel<D, BF, GEN><<<p.units * hkv * p.chunk_splits, 256, 0, stream>>>(a);
+        if (p.chunk_splits > 1) merge_chunk_kernel<D, BF><<<dim3(p.units * hkv, TILE_ROWS / 16), 256, 0, stream>>>(a);
+    }
+    if (p.few_splits) {
+        a.splits = p.few_splits;
+        a.chunk = p.few_chunk;
+        a.part_o = ws + p.chunk_parts * (D + 2);
+        a.part_ml = a.part_o + p.few_parts * D;
+        few_kernel<D, BF, GEN><<<a.b.num_seqs * hkv * p.few_splits, 256, 0, stream>>>(a);
+        if (p.few_splits > 1) merge_few_kernel<D, BF><<<a.b.num_seqs * hkv, 256, 0, stream>>>(a);
+    }
 }
 
 template <int D, bool BF>
-int launch(nnz_ctx *ctx, const AttnArgs &a) {
-    attn_kernel<D, BF><<<dim3(a.b.rows, a.hq), 64, 0, ctx->stream>>>(a);
-    NNZ_LAUNCHED(ctx);
-    return NNZ_OK;
+void start_scores(hipStream_t stream, const Plan &p, const AttnArgs &a, float *ws) {
+    if (a.cap > 0.f || a.slopes) start<D, BF, true>(stream, p, a, ws);
+    else start<D, BF, false>(stream, p, a, ws);
 }
 
 }  // namespace
@@ -81,7 +769,7 @@ int launch(nnz_ctx *ctx, const AttnArgs &a) {
 extern "C" size_t nnz_paged_attention_workspace_bytes(const nnz_paged_kv *kv, const nnz_paged_batch *batch,
                                                       uint32_t num_query_heads) {
     if (paged_fault(kv, batch).code || paged_heads_fault(kv, num_query_heads).code) return 0;
-    return 0;
+    return bytes_of(plan_of(*kv, *batch, num_query_heads), kv->head_dim);
 }
 
 extern "C" int nnz_dispatch_paged_attention(nnz_ctx *ctx, const nnz_paged_kv *kv, const nnz_paged_batch *batch,
@@ -90,6 +778,10 @@ extern "C" int nnz_dispatch_paged_attention(nnz_ctx *ctx, const nnz_paged_kv *kv
     NNZ_CHECK_CTX(ctx);
     if (const PagedFault f = paged_attn_fault(kv, batch, q, output, lse, p); f.code)
         return nnz_fail(ctx, f.code, "paged_attention: %s", f.what);
+    const Plan plan = plan_of(*kv, *batch, p->num_query_heads);
+    const size_t need = bytes_of(plan, kv->head_dim);
+    NNZ_REQUIRE(ctx, need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0), NNZ_EINVAL,
+                "paged_attention: workspace of %zu bytes, 16-byte aligned, needed (%zu given)", need, workspace_bytes);
     NnzDeviceScope scope(ctx);
     AttnArgs a{};
     a.b = paged_view(*kv, *batch);
@@ -105,9 +797,15 @@ extern "C" int nnz_dispatch_paged_attention(nnz_ctx *ctx, const nnz_paged_kv *kv
     a.hq = p->num_query_heads;
     a.G = a.hq / kv->num_kv_heads;
     a.window = p->window;
-    a.scale = p->scale > 0.f ? p->scale : 1.f / sqrtf((float)kv->head_dim);
-    a.cap = p->softcap;
+    const float scale = p->scale > 0.f ? p->scale : 1.f / sqrtf((float)kv->head_dim);
+    a.scale = scale * LOG2E;
+    a.cap = p->softcap * LOG2E;
+    a.cap_in = p->softcap > 0.f ? 2.f * LOG2E * scale / p->softcap : 0.f;
+    a.few = plan.few_splits ? FEW : 0;
     const bool bf = kv->dtype == NNZ_BF16;
-    if (kv->head_dim == 128) return bf ? launch<128, true>(ctx, a) : launch<128, false>(ctx, a);
-    return bf ? launch<64, true>(ctx, a) : launch<64, false>(ctx, a);
+    float *ws = (float *)workspace;
+    if (kv->head_dim == 128) bf ? start_scores<128, true>(ctx->stream, plan, a, ws) : start_scores<128, false>(ctx->stream, plan, a, ws);
+    else bf ? start_scores<64, true>(ctx->stream, plan, a, ws) : start_scores<64, false>(ctx->stream, plan, a, ws);
+    NNZ_LAUNCHED(ctx);
+    return NNZ_OK;
 }

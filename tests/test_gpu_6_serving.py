@@ -350,6 +350,18 @@ def test_attention_agrees_with_the_contiguous_operator(dev):
     assert ((out[0].double() - ref.double()).abs() <= 2 * 2.0 ** -8 * (ref.double().abs() + float(v.abs().max()))).all()
 
 
+def test_attention_refuses_a_short_workspace(dev):
+    c = R.Case([1], [70_001], 8, 2, 128, 64, F16)
+    q = c.normal(c.T, 8, 128)
+    kv = ops.PagedKVCache(dev, c.normal(c.total, 2, 64, 128), c.normal(c.total, 2, 128, 64))
+    n = ops.paged_attention_workspace_bytes(kv, c.batch(ops), 8)
+    assert n > 0
+    for ws in (None, torch.zeros(n - 1, dtype=torch.uint8, device="cuda"),
+               torch.zeros(n + 16, dtype=torch.uint8, device="cuda")[8:]):
+        with pytest.raises(NnzError, match="workspace"):
+            ops.dispatch_paged_attention(dev, kv, c.batch(ops), q, torch.empty_like(q), ws)
+
+
 def test_calls_repeat_bit_for_bit(dev):
     for name in ("decode", "mixed"):
         n, lens, hq, hkv, d, page = ATTENTION[name]
