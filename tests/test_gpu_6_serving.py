@@ -498,6 +498,17 @@ def test_logprobs_of_far_rows(dev):
             assert abs(float(got["lp"][1]) - float(far["lp"][0])) <= 1e-4
 
 
+def test_logprobs_refuses_a_short_workspace(dev):
+    x, tok = torch.randn(1, 151_669, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    n = ops.token_logprobs_workspace_bytes(1, 151_669, 20)
+    assert n > 0
+    ids = torch.zeros(1, 20, dtype=torch.int32, device="cuda")
+    for ws in (None, torch.zeros(n - 1, dtype=torch.uint8, device="cuda"),
+               torch.zeros(n + 16, dtype=torch.uint8, device="cuda")[8:]):
+        with pytest.raises(NnzError, match="workspace"):
+            ops.dispatch_token_logprobs(dev, x, tok, torch.zeros(1, device="cuda"), ws, top_ids=ids)
+
+
 # ------------------------------------------------- used together, as a server does
 class Layer:
     """One attention layer and a 1-bit LM head over paged caches."""
