@@ -8,12 +8,18 @@
 //     t = (x - m) log2(e) / T; x - m before the scale, so that rows of the
 //     type's lowest value stay exact, and w relative to m, so that the entropy
 //     log s - w / s is a sum of terms of one sign;
-//   * per lane the number of ids that come before the token;
-//   * per wave the best top_n so far, one 64-bit key a lane, sorted (value and
-//     complemented id: larger is earlier).  A group of 16 values per lane is
-//     looked at again only if one of them reaches the last of the list, which
-//     after a few groups is rare; what also reaches the top_n-th of the lanes'
-//     maxima is gathered in LDS, 64 at a time sorted and merged into the list.
+//   * the number of ids that come before the token, counted from the compares'
+//     lane masks;
+//   * candidates for the best top_n.  A group of 16 values per lane is looked at
+//     again only if one of them reaches the wave's bound; the bound rises to a
+//     value that top_n of the lanes' maxima reach (top_n values of the row are
+//     no smaller: 16 ballots find its upper half), and what reaches it waits in
+//     LDS with its id.  Should more than 128 wait, they are sorted, 64 at a
+//     time, into a list of keys (value and complemented id: larger is earlier),
+//     whose last bounds what follows.  Ids rise along a wave's part, so that a
+//     full list lets no equal value in: rows of equal values cost one list.
+// At the end the largest of the waves' bounds leaves a few dozen of the block's
+// candidates, which one sort puts in order; the pieces' lists likewise.
 // Keys and counts are integers and the partial sums meet in a fixed order, so a
 // call repeats bit for bit.
 #include "paged_dev.h"
@@ -25,6 +31,7 @@ namespace {
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 
 constexpr uint32_t WAVES = 4, GROUP = 16;   // values of a lane looked at together
+constexpr uint32_t WAITING = 128;           // candidates of a wave that may stay unsorted
 constexpr float LN2 = 0.69314718055994531f, LOG2E = 1.44269504088896341f;
 
 struct LpArgs {
@@ -117,7 +124,24 @@ struct Sums {
         s += o.s;
         w += o.w;
     }
+    __device__ __forceinline__ void join_lanes(float c) {   // the same in every lane
+        rise(wave_max(m), c);
+        s = wave_sum(s);
+        w = wave_sum(w);
+    }
 };
+
+// A value that at least n lanes' x reach, a little below the n-th largest.
+__device__ __forceinline__ float reached_by(float x, uint32_t n) {
+    const uint32_t u = __float_as_uint(x + 0.f), k = u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+    uint32_t f = 0;
+#pragma unroll
+    for (int b = 31; b >= 16; --b) {
+        const uint32_t up = f | 1u << b;
+        f = __builtin_popcountll(__builtin_amdgcn_ballot_w64(k >= up)) >= (int)n ? up : f;
+    }
+    return f <= 0x007FFFFFu ? -INFINITY : __uint_as_float(f >> 31 ? f & 0x7fffffffu : ~f);
+}
 
 // Row-wide results, by one wave: its sums, count and list (lane i holds the
 // i-th key).
@@ -143,8 +167,10 @@ __device__ __forceinline__ void finish(const LpArgs &a, uint32_t row, const Sums
 template <int DT>
 __global__ __launch_bounds__(256) void logprobs_kernel(LpArgs a) {
     constexpr uint32_t ESZ = DT == NNZ_F32 ? 4 : 2, VE = 16 / ESZ, U = GROUP / VE;   // values of a vector, vectors of a group
-    __shared__ uint64_t pool[WAVES][64 * GROUP + 64];   // under 64 keys wait, a group adds 64 GROUP at most
+    __shared__ uint2 pool[WAVES][WAITING + 64 * GROUP + 64];   // value and id; later keys
     __shared__ float4 sums[WAVES];
+    __shared__ float bounds[WAVES];
+    __shared__ uint32_t counts[WAVES];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t row = blockIdx.x / a.pieces, piece = blockIdx.x % a.pieces;
     const unsigned char *const base = (const unsigned char *)a.x + (size_t)row * a.stride * ESZ;
@@ -160,25 +186,32 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LpArgs a) {
     const v4u *const vec = (const v4u *)(base + (size_t)head * ESZ);
 
     Sums t;
-    uint32_t before = 0, held = 0;     // held: keys waiting in the pool
-    uint64_t list = 0, last = 0;       // last: the list's top-th key
-    float last_x = -INFINITY;
-    auto flush = [&]() __attribute__((always_inline)) {   // the pool's last 64 keys join the list
-        const uint32_t n = paged_min(held, 64);
-        held -= n;
+    uint32_t before = 0, held = 0;   // held: candidates waiting in the pool
+    uint64_t list = 0;
+    float bound = -INFINITY;         // what a candidate reaches, or, with `above`, passes
+    bool above = false;
+    auto settle = [&]() __attribute__((always_inline)) {   // LDS written by this wave is there for it
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        const uint64_t k = lane < n ? pool[wave][held + lane] : 0;
-        // sorted falling, read backwards: rising
-        const uint64_t sorted = sort64(k);
-        __builtin_amdgcn_wave_barrier();
-        pool[wave][held + lane] = sorted;
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        list = merge64(list, pool[wave][held + 63 - lane]);
-        __builtin_amdgcn_wave_barrier();
-        last = lane_key(list, a.top - 1);
-        last_x = last ? key_value(last) : -INFINITY;
+    };
+    auto drain = [&]() __attribute__((always_inline)) {   // the pool joins the list
+        settle();
+        for (uint32_t at = 0; at < held; at += 64) {
+            const uint2 f = pool[wave][at + lane];
+            const uint64_t k = sort64(at + lane < held ? order_key(__uint_as_float(f.x), f.y) : 0);
+            settle();
+            pool[wave][at + lane] = make_uint2((uint32_t)k, (uint32_t)(k >> 32));
+            settle();
+            const uint2 r = pool[wave][at + 63 - lane];
+            list = merge64(list, (uint64_t)r.y << 32 | r.x);
+            settle();
+        }
+        held = 0;
+        const uint64_t last = lane_key(list, a.top - 1);
+        if (last) {
+            bound = key_value(last);
+            above = true;
+        }
     };
     // n values of a lane (at most GROUP), ids id(e); those with !on(e) are not there
     auto take = [&](const float *x, auto n_, auto id, auto on, uint32_t first, uint32_t end) __attribute__((always_inline)) {
@@ -195,33 +228,37 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LpArgs a) {
             t.w = fmaf(p, fmaxf(u, -1e30f), t.w);
         }
         if (order) {
+            auto add = [&](bool yes) __attribute__((always_inline)) { before += __builtin_popcountll(__builtin_amdgcn_ballot_w64(yes)); };
             // [first, end): the ids of the whole wave's group
             if (end <= tok && xt == xt) {
 #pragma unroll
-                for (uint32_t e = 0; e < n; ++e) before += on(e) && x[e] >= xt;
+                for (uint32_t e = 0; e < n; ++e) add(on(e) && x[e] >= xt);
             } else if (first > tok && xt == xt) {
 #pragma unroll
-                for (uint32_t e = 0; e < n; ++e) before += on(e) && x[e] > xt;
+                for (uint32_t e = 0; e < n; ++e) add(on(e) && x[e] > xt);
             } else {
 #pragma unroll
                 for (uint32_t e = 0; e < n; ++e)
-                    before += on(e) && (xt != xt ? x[e] == x[e] || id(e) < tok : x[e] > xt || (x[e] == xt && id(e) < tok));
+                    add(on(e) && (xt != xt ? x[e] == x[e] || id(e) < tok : x[e] > xt || (x[e] == xt && id(e) < tok)));
             }
         }
-        if (a.top && __builtin_amdgcn_ballot_w64(mx >= last_x)) {
-            // the top-th largest of the lanes' maxima bounds what can matter
-            const float floor_x = key_value(lane_key(sort64(order_key(mx, 0)), a.top - 1));
+        if (a.top && __builtin_amdgcn_ballot_w64(above ? mx > bound : mx >= bound)) {
+            const float to = reached_by(mx, a.top);
+            if (to > bound) {
+                bound = to;
+                above = false;
+            }
 #pragma unroll
             for (uint32_t e = 0; e < n; ++e) {
-                const uint64_t k = on(e) && x[e] >= floor_x ? order_key(x[e], id(e)) : 0;
-                const uint64_t in = __builtin_amdgcn_ballot_w64(k > last);
+                const bool mine = on(e) && (above ? x[e] > bound : x[e] >= bound);
+                const uint64_t in = __builtin_amdgcn_ballot_w64(mine);
                 if (in) {
                     const uint32_t at = __builtin_amdgcn_mbcnt_hi((uint32_t)(in >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in, 0));
-                    if (k > last) pool[wave][held + at] = k;
+                    if (mine) pool[wave][held + at] = make_uint2(__float_as_uint(x[e]), id(e));
                     held += __builtin_popcountll(in);
                 }
             }
-            while (held >= 64 || (held && !last)) flush();
+            if (held > WAITING) drain();
         }
     };
     auto unpack = [&](const v4u (&r)[U], float *x) __attribute__((always_inline)) {
@@ -266,27 +303,42 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LpArgs a) {
     if (piece == 0 && wave == WAVES - 1) {
         const uint32_t tail = head + nv * VE, left = head + (a.vocab - tail);
         if (left) {
+            above = false;   // its ids may be lower than the list's
             const uint32_t id = lane < head ? lane : tail + (lane - head);
             const bool on = lane < left;
             const float x = on ? load_as_f32<DT>(base, id) : -INFINITY;
             take(&x, std::integral_constant<uint32_t, 1>(), [&](uint32_t) { return id; }, [&](uint32_t) { return on; }, 0u, a.vocab);
         }
     }
-    if (a.top && held) flush();
 
     // the wave's lanes, then the block's waves
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        Sums other;
-        other.m = __shfl_xor(t.m, o);
-        other.s = __shfl_xor(t.s, o);
-        other.w = __shfl_xor(t.w, o);
-        t.join(other, a.c);
-        before += __shfl_xor(before, o);
+    t.join_lanes(a.c);
+    if (lane == 0) {
+        sums[wave] = make_float4(t.m, t.s, t.w, __uint_as_float(before));
+        bounds[wave] = bound;
     }
-    if (lane == 0) sums[wave] = make_float4(t.m, t.s, t.w, __uint_as_float(before));
-    pool[wave][lane] = list;
     __syncthreads();
+    if (a.top) {
+        // what reaches every wave's bound moves to the front of the wave's pool, as keys
+        const float reach = fmaxf(fmaxf(bounds[0], bounds[1]), fmaxf(bounds[2], bounds[3]));
+        uint32_t kept = 0;
+        auto put = [&](uint64_t k) __attribute__((always_inline)) {
+            const uint64_t in = __builtin_amdgcn_ballot_w64(k != 0);
+            const uint32_t at = __builtin_amdgcn_mbcnt_hi((uint32_t)(in >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in, 0));
+            settle();
+            if (k) pool[wave][kept + at] = make_uint2((uint32_t)k, (uint32_t)(k >> 32));
+            settle();
+            kept += __builtin_popcountll(in);
+        };
+        for (uint32_t at = 0; at < held; at += 64) {
+            const uint2 f = pool[wave][at + lane];
+            const float x = __uint_as_float(f.x);
+            put(at + lane < held && x >= reach ? order_key(x, f.y) : 0);
+        }
+        if (__builtin_amdgcn_ballot_w64(list != 0)) put(lane < a.top ? list : 0);
+        if (lane == 0) counts[wave] = kept;
+        __syncthreads();
+    }
     if (wave) return;
 #pragma unroll
     for (uint32_t i = 1; i < WAVES; ++i) {
@@ -297,7 +349,20 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LpArgs a) {
         other.w = f.z;
         t.join(other, a.c);
         before += __float_as_uint(f.w);
-        if (a.top) list = merge64(list, pool[i][63 - lane]);
+    }
+    if (a.top) {
+        const uint32_t n0 = counts[0], n1 = n0 + counts[1], n2 = n1 + counts[2], n3 = n2 + counts[3];
+        list = 0;
+        for (uint32_t j = 0; j < n3; j += 64) {
+            const uint32_t i = j + lane;
+            const uint2 f = i < n0 ? pool[0][i] : i < n1 ? pool[1][i - n0] : i < n2 ? pool[2][i - n1] : pool[3][i < n3 ? i - n2 : 0];
+            uint64_t k = sort64(i < n3 ? (uint64_t)f.y << 32 | f.x : 0);
+            if (j) {   // two falling lists: the second one backwards
+                const uint32_t lo = __shfl((uint32_t)k, 63 - lane), hi = __shfl((uint32_t)(k >> 32), 63 - lane);
+                k = merge64(list, (uint64_t)hi << 32 | lo);
+            }
+            list = k;
+        }
     }
     if (a.pieces == 1) {
         finish(a, row, t, before, list, xt, named);
@@ -307,55 +372,82 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LpArgs a) {
     if (lane < a.top) a.part_keys[(size_t)blockIdx.x * a.top + lane] = list;
 }
 
-// The pieces of a row joined: 16 waves take them in turn, then pair by pair.
+// The pieces of a row joined: sums by wave 0, a piece a lane; keys that reach
+// every piece's last one, a few dozen, gathered in LDS and sorted.  (Where
+// pieces are equal in value the last keys differ by id, so that the bound, the
+// largest of them, leaves fewer than 64 of each.)
 template <int DT>
-__global__ __launch_bounds__(1024) void logprobs_join_kernel(LpArgs a) {
-    __shared__ uint64_t lists[16][64];
-    __shared__ float4 sums[16];
-    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = blockIdx.x;
+__global__ __launch_bounds__(256) void logprobs_join_kernel(LpArgs a) {
+    extern __shared__ uint64_t kept[];   // [pieces * top]
+    __shared__ uint64_t reach[WAVES];
+    __shared__ uint32_t count;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), row = blockIdx.x;
     const uint32_t tok = a.tokens[row];
     const bool named = tok < a.vocab;
     const float xt = named ? load_as_f32<DT>(a.x, (size_t)row * a.stride + tok) : 0.f;
+    const float4 *const part = a.part + (size_t)row * a.pieces;
+    const uint64_t *const keys = a.part_keys + (size_t)row * a.pieces * a.top;
+    if (a.top) {
+        uint64_t k = 0;
+        for (uint32_t p = tid; p < a.pieces; p += 256) {
+            const uint64_t last = keys[(size_t)p * a.top + a.top - 1];
+            k = last > k ? last : k;
+        }
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint64_t v = __shfl_xor((unsigned long long)k, o);
+            k = v > k ? v : k;
+        }
+        if (lane == 0) reach[wave] = k;
+        if (tid == 0) count = 0;
+        __syncthreads();
+#pragma unroll
+        for (uint32_t i = 0; i < WAVES; ++i) k = reach[i] > k ? reach[i] : k;
+        for (uint32_t i = tid; i < a.pieces * a.top; i += 256) {
+            const uint64_t v = keys[i];
+            if (v && v >= k) kept[atomicAdd(&count, 1u)] = v;   // any order: they are sorted next
+        }
+        __syncthreads();
+    }
+    if (wave) return;
     Sums t;
     uint32_t before = 0;
-    uint64_t list = 0;
-    auto add = [&](float4 f) {
+    for (uint32_t p = lane; p < a.pieces; p += 64) {
+        const float4 f = part[p];
         Sums o;
         o.m = f.x;
         o.s = f.y;
         o.w = f.z;
         t.join(o, a.c);
         before += __float_as_uint(f.w);
-    };
-    for (uint32_t p = wave; p < a.pieces; p += 16) {
-        const size_t at = (size_t)row * a.pieces + p;
-        add(a.part[at]);
-        if (a.top) list = merge64(list, 63 - lane < a.top ? a.part_keys[at * a.top + 63 - lane] : 0);
     }
-    for (uint32_t half = 8; half; half /= 2) {
-        if (wave >= half && wave < 2 * half) {
-            lists[wave][lane] = list;
-            if (lane == 0) sums[wave] = make_float4(t.m, t.s, t.w, __uint_as_float(before));
+    t.join_lanes(a.c);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) before += __shfl_xor(before, o);
+    uint64_t list = 0;
+    if (a.top)
+        for (uint32_t j = 0; j < count; j += 64) {
+            uint64_t k = sort64(j + lane < count ? kept[j + lane] : 0);
+            if (j) {
+                const uint32_t lo = __shfl((uint32_t)k, 63 - lane), hi = __shfl((uint32_t)(k >> 32), 63 - lane);
+                k = merge64(list, (uint64_t)hi << 32 | lo);
+            }
+            list = k;
         }
-        __syncthreads();
-        if (wave < half) {
-            add(sums[wave + half]);
-            list = merge64(list, lists[wave + half][63 - lane]);
-        }
-    }
-    if (wave == 0) finish(a, row, t, before, list, xt, named);
+    finish(a, row, t, before, list, xt, named);
 }
 
 // Blocks for about four per CU, each with a group of values per lane at least.
+// At most 96: the join's keys (64 each) stay within 48 KB of LDS.
 uint32_t pieces_of(uint32_t rows, uint32_t vocab) {
     const uint32_t want = std::max(1u, 1024u / rows), most = std::max(1u, vocab / (WAVES * 64 * GROUP));
-    return std::min(want, most);
+    return std::min({want, most, 96u});
 }
 
 template <int DT>
 void start(hipStream_t stream, const LpArgs &a, uint32_t rows) {
     logprobs_kernel<DT><<<rows * a.pieces, 256, 0, stream>>>(a);
-    if (a.pieces > 1) logprobs_join_kernel<DT><<<rows, 1024, 0, stream>>>(a);
+    if (a.pieces > 1) logprobs_join_kernel<DT><<<rows, 256, (size_t)a.pieces * a.top * 8, stream>>>(a);
 }
 
 }  // namespace
