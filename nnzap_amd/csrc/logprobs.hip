@@ -174,16 +174,25 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LpArgs a) {
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t row = blockIdx.x / a.pieces, piece = blockIdx.x % a.pieces;
     const unsigned char *const base = (const unsigned char *)a.x + (size_t)row * a.stride * ESZ;
-    const uint32_t tok = a.tokens[row];
-    const bool named = tok < a.vocab, order = named && a.rank;
-    const float xt = named ? load_as_f32<DT>(base, tok) : 0.f;
-
     // 16-byte vectors from the first aligned one on; what is left over before
     // and after them (under 2 VE values) is piece 0's
     const uint32_t head = paged_min(a.vocab, (uint32_t)(-(intptr_t)base & 15) / ESZ);
     const uint32_t nv = (a.vocab - head) / VE;
     const uint32_t v0 = (uint32_t)((uint64_t)nv * piece / a.pieces), v1 = (uint32_t)((uint64_t)nv * (piece + 1) / a.pieces);
     const v4u *const vec = (const v4u *)(base + (size_t)head * ESZ);
+
+    constexpr uint32_t STEP = 64 * U;   // vectors of a wave's group
+    uint32_t v = v0 + wave * STEP;
+    v4u r[U];
+    auto load = [&](uint32_t at) __attribute__((always_inline)) {
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) r[u] = __builtin_nontemporal_load(vec + at + 64 * u + lane);
+    };
+    if (v + STEP <= v1) load(v);   // before the token's value, which takes two rounds to memory
+
+    const uint32_t tok = a.tokens[row];
+    const bool named = tok < a.vocab, order = named && a.rank;
+    const float xt = named ? load_as_f32<DT>(base, tok) : 0.f;
 
     Sums t;
     uint32_t before = 0, held = 0;   // held: candidates waiting in the pool
@@ -274,15 +283,7 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LpArgs a) {
                 }
             }
     };
-    constexpr uint32_t STEP = 64 * U;   // vectors of a wave's group
-    uint32_t v = v0 + wave * STEP;
-    v4u r[U];
-    auto load = [&](uint32_t at) __attribute__((always_inline)) {
-#pragma unroll
-        for (uint32_t u = 0; u < U; ++u) r[u] = __builtin_nontemporal_load(vec + at + 64 * u + lane);
-    };
     auto id_of = [&](uint32_t at, uint32_t e) { return head + (at + 64 * (e / VE) + lane) * VE + e % VE; };
-    if (v + STEP <= v1) load(v);
     for (; v + STEP <= v1; v += WAVES * STEP) {   // whole groups, the next one's loads in flight
         float x[GROUP];
         unpack(r, x);

@@ -3,6 +3,8 @@
 // query and key, and the copy of K and V into their pages.
 #include "paged_dev.h"
 
+#include <algorithm>
+
 namespace {
 
 struct AppendArgs {
@@ -17,57 +19,146 @@ struct AppendArgs {
     float eps;
 };
 
-// One wave per (row, head of q, k or v); lane l holds dims l, l + 64, ...
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+
+// Bound by the bytes of q, k and v, read and written once.  A block takes the
+// rows of one aligned group of 8 positions of a sequence (they lie in one page)
+// and a share of the heads: 8 dims of a row a thread, so that norm and rotation
+// stay within 16 (8 at head_dim 64) lanes, with the group's cosines and sines
+// computed once into LDS.  V goes to its transposed page two dims a lane, all
+// positions of the group in registers: whole groups are two 16-byte stores.
 template <int D, bool BF>
-__global__ __launch_bounds__(64) void append_kernel(AppendArgs a) {
-    const uint32_t row = blockIdx.x, head = blockIdx.y, l = threadIdx.x;
-    uint32_t s = 0;
-    while (s < a.b.num_seqs && a.b.starts[s + 1] <= row) ++s;
-    if (s == a.b.num_seqs) return;
+__global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
+    constexpr uint32_t LPR = D / 8, SETS = 256 / LPR;   // lanes of a row, rows at a time
+    __shared__ float2 cs[8][D / 2];
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    uint32_t s = blockIdx.x, g = 0;
+    if (a.b.max_q > 1) {
+        if (!paged_find(a.b.num_seqs, blockIdx.x, &s, &g,
+                        [&](uint32_t i) { return paged_groups(paged_seq(a.b, i), a.b); }))
+            return;
+    }
     const PagedSeq sq = paged_seq(a.b, s);
-    if (row < sq.row0 || row - sq.row0 >= sq.n || row - sq.row0 >= a.b.max_q) return;
-    const int32_t p = sq.first + (int32_t)(row - sq.row0);
-    if (p < 0) return;
-    const uint32_t page = paged_page(a.b, s, (uint32_t)p), slot = (uint32_t)p & ((1u << a.b.shift) - 1);
-    if (head >= a.hq && page >= a.b.num_pages) return;
-    __shared__ float x[D];
-    if (head >= a.hq + a.b.hkv) {
-        const uint32_t h = head - a.hq - a.b.hkv;
-        const uint16_t *src = a.v + row * a.v_stride + h * D;
-        uint16_t *dst = a.v_pages + ((((size_t)page * a.b.hkv + h) * D) << a.b.shift) + slot;
-        for (uint32_t d = l; d < D; d += 64) dst[(size_t)d << a.b.shift] = src[d];
-        return;
+    uint32_t i0, i1;
+    paged_group_rows(sq, a.b, paged_first_group(sq) + g, &i0, &i1);
+    if (i0 >= i1) return;
+    const uint32_t nt = i1 - i0, p0 = (uint32_t)(sq.first + (int32_t)i0);
+    const uint32_t page = paged_entry(a.b, s, p0, true), slot = p0 & ((1u << a.b.shift) - 1);
+    const bool paged = page < a.b.num_pages;
+    const size_t row0 = sq.row0 + i0;
+
+    // rows of heads: set i of the block is token i % np of heads i / np, ...
+    const uint32_t lg = nt > 4 ? 3 : nt > 2 ? 2 : nt > 1 ? 1 : 0, set = tid / LPR, col = tid % LPR;
+    const uint32_t tok = set & ((1u << lg) - 1), step = SETS >> lg, heads = a.hq + (paged ? a.b.hkv : 0);
+    const bool on = tok < nt;
+    const size_t row = row0 + (on ? tok : 0);
+    auto source = [&](uint32_t h) {
+        return (h < a.hq ? a.q + row * a.q_stride + h * D : a.k + row * a.k_stride + (h - a.hq) * D) + 8 * col;
+    };
+    uint32_t h = (set >> lg) + blockIdx.y * step;
+    const uint32_t hstep = step * gridDim.y;
+    v4u r = {};
+    if (on && h < heads) r = *(const v4u *)source(h);
+
+    // V, two dims a lane
+    constexpr uint32_t LPV = D / 2, HW = 64 / LPV;
+    const uint32_t vd = 2 * (lane % LPV);
+    if (paged) {
+        for (uint32_t hv = (blockIdx.y * 4 + wave) * HW + lane / LPV; hv < a.b.hkv; hv += 4 * HW * gridDim.y) {
+            const uint16_t *src = a.v + row0 * a.v_stride + hv * D + vd;
+            uint16_t *dst = a.v_pages + ((((size_t)page * a.b.hkv + hv) * D + vd) << a.b.shift) + slot;
+            uint32_t x[8];
+#pragma unroll
+            for (uint32_t t = 0; t < 8; ++t)
+                if (t < nt) x[t] = *(const uint32_t *)(src + t * a.v_stride);
+            if (nt == 8) {
+                v4u lo, hi;
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) {
+                    lo[i] = (x[2 * i] & 0xFFFFu) | x[2 * i + 1] << 16;
+                    hi[i] = x[2 * i] >> 16 | (x[2 * i + 1] & 0xFFFF0000u);
+                }
+                *(v4u *)dst = lo;
+                *(v4u *)(dst + ((size_t)1 << a.b.shift)) = hi;
+            } else {
+#pragma unroll
+                for (uint32_t t = 0; t < 8; ++t)
+                    if (t < nt) {
+                        dst[t] = (uint16_t)x[t];
+                        dst[((size_t)1 << a.b.shift) + t] = (uint16_t)(x[t] >> 16);
+                    }
+            }
+        }
     }
-    const bool isq = head < a.hq;
-    const uint32_t h = isq ? head : head - a.hq;
-    const uint16_t *src = isq ? a.q + row * a.q_stride + h * D : a.k + row * a.k_stride + h * D;
-    const float *w = isq ? a.q_scale : a.k_scale;
-    float ss = 0.f;
-    for (uint32_t d = l; d < D; d += 64) {
-        x[d] = paged_load<BF>(src[d]);
-        ss += x[d] * x[d];
-    }
-    if (w) {
-        const float r = rsqrtf(wave_sum(ss) / (float)D + a.eps);
-        for (uint32_t d = l; d < D; d += 64) x[d] = x[d] * r * w[d];
-    }
+
+    if ((tid & 63) < a.half)
+        for (uint32_t t = tid >> 6; t < nt; t += 4) cs[t][tid & 63] = paged_cos_sin((int32_t)(p0 + t), a.inv_freq, a.log2_step, tid & 63);
     __syncthreads();
-    for (uint32_t k = l; k < a.half; k += 64) {
-        const uint32_t d0 = a.halves ? k : 2 * k, d1 = a.halves ? k + a.half : 2 * k + 1;
-        const float2 cs = paged_cos_sin(p, a.inv_freq, a.log2_step, k);
-        const float u = x[d0], v = x[d1];
-        x[d0] = u * cs.x - v * cs.y;
-        x[d1] = u * cs.y + v * cs.x;
+    const uint32_t d0 = 8 * col, hl = a.half / 8;   // first dim; lanes of half the rotated dims
+    for (; h < heads; h += hstep) {
+        v4u next = {};
+        if (on && h + hstep < heads) next = *(const v4u *)source(h + hstep);
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = paged_load<BF>((uint16_t)(r[e >> 1] >> (16 * (e & 1))));
+        const float *w = h < a.hq ? a.q_scale : a.k_scale;
+        if (w) {
+            float ss = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
+            ss += dpp_move<DPP_XOR1>(ss, 0.f);
+            ss += dpp_move<DPP_XOR2>(ss, 0.f);
+            ss += dpp_move<DPP_ROW_HALF_MIRROR>(ss, 0.f);
+            if constexpr (LPR == 16) ss += dpp_move<DPP_ROW_MIRROR>(ss, 0.f);
+            const float f = rsqrtf(ss / (float)D + a.eps);
+            const float4 wa = *(const float4 *)(w + d0), wb = *(const float4 *)(w + d0 + 4);
+            x[0] *= f * wa.x, x[1] *= f * wa.y, x[2] *= f * wa.z, x[3] *= f * wa.w;
+            x[4] *= f * wb.x, x[5] *= f * wb.y, x[6] *= f * wb.z, x[7] *= f * wb.w;
+        }
+        if (a.halves) {
+            const bool first = d0 < a.half, in = d0 < 2 * a.half;   // whole lanes: half is a multiple of 8
+            const int from = (int)(first ? lane + hl : lane - hl);
+            const uint32_t k0 = first ? d0 : d0 - a.half;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float y = __shfl(x[e], in ? from : (int)lane);
+                if (in) {
+                    const float2 c = cs[on ? tok : 0][k0 + e];
+                    x[e] = fmaf(x[e], c.x, first ? -y * c.y : y * c.y);
+                }
+            }
+        } else if (d0 < 2 * a.half) {
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                const float2 c = cs[on ? tok : 0][(d0 + e) / 2];
+                const float u = x[e], v = x[e + 1];
+                x[e] = fmaf(u, c.x, -v * c.y);
+                x[e + 1] = fmaf(u, c.y, v * c.x);
+            }
+        }
+        v4u y;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            y[i] = (uint32_t)paged_round<BF>(x[2 * i]) | (uint32_t)paged_round<BF>(x[2 * i + 1]) << 16;
+        if (on) {
+            uint16_t *dst = h < a.hq ? a.q_out + row * a.qo_stride + h * D
+                                     : a.k_pages + (((((size_t)page * a.b.hkv + h - a.hq) << a.b.shift) + slot + tok) * D);
+            *(v4u *)(dst + d0) = y;
+        }
+        r = next;
     }
-    __syncthreads();
-    uint16_t *dst = isq ? a.q_out + row * a.qo_stride + h * D
-                        : a.k_pages + (((((size_t)page * a.b.hkv + h) << a.b.shift) + slot) * D);
-    for (uint32_t d = l; d < D; d += 64) dst[d] = paged_round<BF>(x[d]);
 }
 
 template <int D, bool BF>
 int launch(nnz_ctx *ctx, const AppendArgs &a) {
-    append_kernel<D, BF><<<dim3(a.b.rows, a.hq + 2 * a.b.hkv), 64, 0, ctx->stream>>>(a);
+    // Groups of 8 positions, an upper bound; the heads are shared out until
+    // there are about 1024 blocks, down to four rows of heads for a thread (one
+    // for single tokens, whose blocks take 16 heads at a time).
+    const uint64_t groups = std::min<uint64_t>((uint64_t)a.b.rows / 8 + 2ull * a.b.num_seqs,
+                                               (uint64_t)a.b.num_seqs * paged_groups_max(a.b.max_q));
+    const uint32_t heads = a.hq + a.b.hkv, most = ceil_div(heads, a.b.max_q > 1 ? 8 : 16);
+    const uint32_t shares = std::min(most, (uint32_t)std::max<uint64_t>(1, 1024 / groups));
+    append_kernel<D, BF><<<dim3((uint32_t)groups, shares), 256, 0, ctx->stream>>>(a);
     NNZ_LAUNCHED(ctx);
     return NNZ_OK;
 }

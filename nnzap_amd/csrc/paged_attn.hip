@@ -10,13 +10,14 @@
 // it as its B operand: the weights never move between lanes.  V's pages are
 // transposed, so V^T's A operand is 16 contiguous bytes of a page.
 //
-//   few_kernel    at most 16 rows (single tokens, drafts): bound by the bytes
-//                 of K and V, which go straight from memory into the operand
-//                 registers, each byte once; keys are split over waves and
-//                 blocks, merge_few_kernel joins the blocks' parts.
-//   chunk_kernel  more rows (chunks of prompts): bound by the matrix cores and
-//                 the softmax's vector work beside them; 128 rows a block, K
-//                 and V tiles of 64 keys in LDS, two buffers.
+//   few_part    at most 16 rows (single tokens, drafts): bound by the bytes of
+//               K and V, which go straight from memory into the operand
+//               registers, each byte once; keys are split over waves and blocks;
+//   chunk_part  more rows (chunks of prompts): bound by the matrix cores and the
+//               softmax's vector work beside them; 128 rows a block, K and V
+//               tiles of 64 keys in LDS, two buffers; keys are split over blocks
+//               where there are few rows.
+// join_kernel joins what blocks computed of one row.
 //
 // The softmax is the online one in base 2: sums are kept relative to a
 // reference M per row, which follows the row's maximum only when that runs
@@ -26,6 +27,7 @@
 #include "paged_dev.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 
@@ -38,9 +40,9 @@ typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf2v __attribute__((ext_vector_type(2)));
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 
-constexpr uint32_t FEW = 16;      // most rows of few_kernel
+constexpr uint32_t FEW = 16;      // most rows of few_part
 constexpr uint32_t TILE_ROWS = 128;
-constexpr uint32_t KT = 64;       // keys per tile of chunk_kernel
+constexpr uint32_t KT = 64;       // keys per tile of chunk_part
 constexpr float LN2 = 0.69314718055994531f, LOG2E = 1.44269504088896341f;
 
 struct AttnArgs {
@@ -54,10 +56,14 @@ struct AttnArgs {
     uint32_t hq, G, window;
     float scale;          // of the scores, times log2 e
     float cap_in, cap;    // softcap: cap * tanh(x) with 2 log2(e) x = cap_in * (q . k); cap times log2 e
-    uint32_t few;         // sequences of at most this many rows are few_kernel's
-    uint32_t units;       // row tiles of the whole batch, an upper bound
-    uint32_t splits, chunk;
-    float *part_o, *part_ml;
+    // Sequences of at most `few` rows (0: none) are few_part's: keys in chunks of
+    // few_steps steps, at most few_splits of them, a block each, few_blocks in all.
+    uint32_t few, few_splits, few_steps, few_blocks;
+    // The others' are chunk_part's: `units` row tiles in the whole batch, an upper
+    // bound, keys in chunks of chunk_tiles tiles, at most chunk_splits of them.
+    uint32_t units, chunk_splits, chunk_tiles;
+    uint32_t few_rows;              // most rows of a sequence in few_part
+    float *few_o, *few_ml, *chunk_o, *chunk_ml;
 };
 
 template <bool BF>
@@ -83,47 +89,25 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     else return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, half2v));
 }
 
-// Nonzero if any of the eight values is NaN or infinite.
+// A step that some rows see only in part must not let a hidden key's weight of
+// 0 meet NaN or infinities in V.  Such steps multiply by V without those;
+// where one was met (odd), the rows that do see it get it afterwards, in a pass
+// of its own over the wave's keys (odd_value).
 template <bool BF>
-__device__ __forceinline__ uint32_t nonfinite(v4u v) {
+__device__ __forceinline__ v4u finite_part(v4u v, uint32_t &odd) {
     constexpr uint32_t EXP = BF ? 0x7F807F80u : 0x7C007C00u, STEP = BF ? 0x00800080u : 0x04000400u;
-    uint32_t bad = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) bad |= (v[i] & EXP) + STEP;
-    return bad & 0x80008000u;
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t t = ((v[i] & EXP) + STEP) & 0x80008000u;   // of each half: all exponent bits set
+        odd |= t;
+        v[i] &= ~((t - (t >> 15)) | t);
+    }
+    return v;
 }
-
-// O^T += V^T . P^T for a V with NaN or infinities, where some rows see only a
-// part of the step: a hidden key's weight of 0 must not meet them, while the
-// rows that do see it get what they should.  The product takes V without them;
-// products of their places (1 each) with the keys' visibility (bit e of vis is
-// this lane's key e) say which sums they belong to.
-template <bool BF, class ACC, class MFMA>
-__device__ __forceinline__ void add_nonfinite(ACC &o, v4u v, v4u p, uint32_t vis, MFMA mfma) {
-    constexpr uint32_t EXP = BF ? 0x7F80u : 0x7C00u, ONE = BF ? 0x3F80u : 0x3C00u;
-    v4u seen = {}, x = {};
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const uint32_t sh = 16 * (e & 1), u = v[e >> 1] >> sh & 0xFFFFu;
-        seen[e >> 1] |= (vis >> e & 1 ? ONE : 0u) << sh;
-        x[e >> 1] |= ((u & 0x7FFFu) < EXP ? u : 0u) << sh;
-    }
-    o = mfma(x, p, o);
-    for (int kind = 0; kind < 3; ++kind) {   // NaN, +inf, -inf
-        const uint32_t first = kind == 0 ? EXP + 1 : kind == 1 ? EXP : EXP | 0x8000u;
-        const uint32_t mask = kind == 0 ? 0x7FFFu : 0xFFFFu, last = kind == 0 ? 0x7FFFu : first;
-        const float val = kind == 0 ? __builtin_nanf("") : kind == 1 ? INFINITY : -INFINITY;
-        x = (v4u){0, 0, 0, 0};
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const uint32_t sh = 16 * (e & 1), u = (v[e >> 1] >> sh) & mask;
-            x[e >> 1] |= (u >= first && u <= last ? ONE : 0u) << sh;
-        }
-        ACC t = {};
-        t = mfma(x, seen, t);
-#pragma unroll
-        for (int e = 0; e < (int)(sizeof(ACC) / 4); ++e) o[e] += t[e] > 0.f ? val : 0.f;
-    }
+template <bool BF>
+__device__ __forceinline__ float odd_value(uint16_t v, bool seen) {
+    const float f = paged_load<BF>(v);
+    return seen && !(fabsf(f) < INFINITY) ? f : 0.f;
 }
 
 // A score as the definition has it, in log2 units (capped scores or a bias);
@@ -133,16 +117,6 @@ __device__ __forceinline__ float general_score(const AttnArgs &a, float s, float
     if (a.cap > 0.f)   // tanh(x) = 1 - 2 / (e^2x + 1)
         t = a.cap * fmaf(-2.f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(a.cap_in * s) + 1.f), 1.f);
     return fmaf(-slope, fabsf((float)distance), t);
-}
-
-// A table entry through the scalar cache (the table does not change while the
-// kernel runs); num_pages where there is no page or the keys are not wanted.
-__device__ __forceinline__ uint32_t page_at(const PagedView &b, uint32_t s, uint32_t key, bool wanted) {
-    const uint32_t e = key >> b.shift;
-    if (!wanted || e >= b.width) return b.num_pages;
-    typedef const uint32_t __attribute__((address_space(4))) *table_t;
-    const table_t t = (table_t)(uintptr_t)(b.table + (size_t)s * b.width);
-    return paged_min(t[e], b.num_pages);
 }
 
 // ---------------------------------------------------------------- few rows
@@ -157,13 +131,18 @@ struct FewStep {
     uint32_t bad;   // groups of 16 keys without a page
 };
 
+template <int D>
+struct FewShared {
+    float4v o[4][D / 16][64];
+    float m[4][16], l[4][16];
+};
+
 template <int D, bool BF, bool GEN>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void few_kernel(AttnArgs a) {
+__device__ __forceinline__ void few_part(const AttnArgs &a, uint32_t block, FewShared<D> &sh) {
     constexpr int NKS = D / 32, NDT = D / 16;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, c = lane & 15;
-    const uint32_t hkv = a.b.hkv, kvh = blockIdx.x % hkv, z = blockIdx.x / hkv % a.splits,
-                   s = blockIdx.x / hkv / a.splits;
+    const uint32_t hkv = a.b.hkv, kvh = block % hkv, z = block / hkv % a.few_splits, s = block / hkv / a.few_splits;
     const PagedSeq sq = paged_seq(a.b, s);
     const uint32_t n = paged_min(sq.n, a.b.max_q), R = n * a.G;
     if (R == 0 || R > FEW) return;
@@ -171,9 +150,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void f
     const PagedSpan sp0 = paged_span(sq.first, sq.len, prefix, a.window);
     const PagedSpan sp1 = paged_span(sq.first + (int32_t)n - 1, sq.len, prefix, a.window);
     const uint32_t lo = sp0.lo & ~31u, hi = sp1.hi, steps = hi > lo ? (hi - lo + 31) / 32 : 0;
-    const uint32_t nz = steps > a.chunk ? (steps + a.chunk - 1) / a.chunk : 1;
+    const uint32_t nz = steps > a.few_steps ? (steps + a.few_steps - 1) / a.few_steps : 1;
     if (z >= nz) return;
-    const uint32_t st1 = paged_min(steps, (z + 1) * a.chunk);
+    const uint32_t st1 = paged_min(steps, (z + 1) * a.few_steps);
 
     const uint32_t r = paged_min((uint32_t)c, R - 1), tok = r / a.G, head = kvh * a.G + r % a.G;
     const int32_t pos = sq.first + (int32_t)tok;
@@ -189,7 +168,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void f
     const uint32_t pmask = (1u << a.b.shift) - 1;
     auto load = [&](FewStep<D, BF> &f, uint32_t st) __attribute__((always_inline)) {
         const uint32_t k0 = lo + 32 * st;
-        uint32_t pa = page_at(a.b, s, k0, true), pb = page_at(a.b, s, k0 + 16, k0 + 16 < hi);
+        uint32_t pa = paged_entry(a.b, s, k0, true), pb = paged_entry(a.b, s, k0 + 16, k0 + 16 < hi);
         f.bad = (pa == a.b.num_pages ? 1u : 0u) | (pb == a.b.num_pages ? 2u : 0u);
         pa = f.bad & 1 ? 0u : pa;   // any page: the keys are masked
         pb = f.bad & 2 ? 0u : pb;
@@ -212,6 +191,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void f
     for (int dt = 0; dt < NDT; ++dt) o[dt] = (float4v){0.f, 0.f, 0.f, 0.f};
     const float cs = GEN ? 1.f : a.scale, ahead = 8.f / cs;
     float m = -INFINITY, nm = 0.f, l = 0.f;   // reference score, minus it in log2 units, sum of this lane's weights
+    uint32_t odd = 0;
+    auto in_part = [&](uint32_t k0, uint32_t bad) { return k0 < sp1.lo || k0 + 32 > sp0.hi || bad; };   // wave-uniform
     auto compute = [&](const FewStep<D, BF> &f, uint32_t st) __attribute__((always_inline)) {
         const uint32_t k0 = lo + 32 * st;
         float sc[8];
@@ -228,15 +209,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void f
 #pragma unroll
             for (int e = 0; e < 8; ++e) sc[e] = general_score(a, sc[e], slope, pos - (int32_t)(key + e));
         }
-        const bool masked = k0 < sp1.lo || k0 + 32 > sp0.hi || f.bad;   // wave-uniform
-        uint32_t vis = 0xFF;
+        const bool masked = in_part(k0, f.bad);
         if (masked) {
             const bool on = !(f.bad >> (g >> 1) & 1);
-            vis = 0;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) vis |= (on && key + e >= sp.lo && key + e < sp.hi ? 1u : 0u) << e;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) sc[e] = vis >> e & 1 ? sc[e] : -INFINITY;
+            for (int e = 0; e < 8; ++e) sc[e] = on && key + e >= sp.lo && key + e < sp.hi ? sc[e] : -INFINITY;
         }
         float mx = sc[0];
 #pragma unroll
@@ -263,19 +240,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void f
         for (int i = 0; i < 4; ++i) p[i] = pack2<BF>(sc[2 * i], sc[2 * i + 1]);
         if (masked) {
 #pragma unroll
-            for (int dt = 0; dt < NDT; ++dt) {
-                if (__builtin_amdgcn_ballot_w64(nonfinite<BF>(f.v[dt]) != 0))   // wave-uniform, rare
-                    add_nonfinite<BF>(o[dt], f.v[dt], p, vis, mfma16<BF>);
-                else
-                    o[dt] = mfma16<BF>(f.v[dt], p, o[dt]);
-            }
+            for (int dt = 0; dt < NDT; ++dt) o[dt] = mfma16<BF>(finite_part<BF>(f.v[dt], odd), p, o[dt]);
         } else {
 #pragma unroll
             for (int dt = 0; dt < NDT; ++dt) o[dt] = mfma16<BF>(f.v[dt], p, o[dt]);
         }
     };
 
-    uint32_t st = z * a.chunk + (uint32_t)w;
+    uint32_t st = z * a.few_steps + (uint32_t)w;
     if (st < st1) {   // wave-uniform, all of it
         FewStep<D, BF> f0, f1;
         load(f0, st);
@@ -290,28 +262,45 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void f
             if (st >= st1) break;
         }
     }
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(odd != 0) != 0, 0)) {   // wave-uniform
+        for (st = z * a.few_steps + (uint32_t)w; st < st1; st += 4) {
+            const uint32_t k0 = lo + 32 * st;
+            const bool hole = paged_entry(a.b, s, k0, true) == a.b.num_pages ||
+                              paged_entry(a.b, s, k0 + 16, k0 + 16 < hi) == a.b.num_pages;
+            if (!in_part(k0, hole)) continue;   // whole steps had V as it is
+            for (uint32_t key = k0; key < k0 + 32; ++key) {
+                const uint32_t page = paged_entry(a.b, s, key, key < hi);
+                if (page == a.b.num_pages) continue;
+                const uint16_t *vp = a.v + ((((size_t)page * hkv + kvh) * D) << a.b.shift) + (key & pmask);
+                const bool seen = key >= sp.lo && key < sp.hi;
+#pragma unroll
+                for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        o[dt][e] += odd_value<BF>(vp[(size_t)(16 * dt + 4 * g + e) << a.b.shift], seen);
+            }
+        }
+    }
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
 
     // the four waves' parts, relative to the largest reference
-    __shared__ float4v so[4][NDT][64];
-    __shared__ float sm[4][16], sl[4][16];
 #pragma unroll
-    for (int dt = 0; dt < NDT; ++dt) so[w][dt][lane] = o[dt];
+    for (int dt = 0; dt < NDT; ++dt) sh.o[w][dt][lane] = o[dt];
     if (g == 0) {
-        sm[w][c] = m == -INFINITY ? -INFINITY : -nm;
-        sl[w][c] = l;
+        sh.m[w][c] = m == -INFINITY ? -INFINITY : -nm;
+        sh.l[w][c] = l;
     }
     __syncthreads();
-    float M = sm[0][c], wt[4];
+    float M = sh.m[0][c], wt[4];
 #pragma unroll
-    for (int i = 1; i < 4; ++i) M = fmaxf(M, sm[i][c]);
+    for (int i = 1; i < 4; ++i) M = fmaxf(M, sh.m[i][c]);
     l = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        wt[i] = sm[i][c] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sm[i][c] - M);
-        l += wt[i] * sl[i][c];
-        if (sl[i][c] != sl[i][c]) l = sl[i][c];
+        wt[i] = sh.m[i][c] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sh.m[i][c] - M);
+        l += wt[i] * sh.l[i][c];
+        if (sh.l[i][c] != sh.l[i][c]) l = sh.l[i][c];
     }
     const bool mine = (uint32_t)c < R;
     if (nz == 1) {
@@ -322,8 +311,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void f
             if (dt % 4 != w) continue;
             float4v t = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (wt[i] != 0.f) t += so[i][dt][lane] * wt[i];
+            for (int i = 0; i < 4; ++i) t += sh.o[i][dt][lane] * wt[i];
             if (l != l) t = (float4v){l, l, l, l};
             if (mine)
                 *(uint2 *)(op + 16 * dt) = make_uint2(pack2<BF>(t[0] * inv, t[1] * inv), pack2<BF>(t[2] * inv, t[3] * inv));
@@ -332,70 +320,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void f
             a.lse[(size_t)(sq.row0 + tok) * a.hq + head] = l == 0.f ? -INFINITY : (M + __builtin_amdgcn_logf(l)) * LN2;
         return;
     }
-    const size_t part = (((size_t)s * hkv + kvh) * a.splits + z) * FEW + (uint32_t)c;
+    const size_t part = (((size_t)s * hkv + kvh) * a.few_splits + z) * a.few_rows + (uint32_t)c;
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt) {
         if (dt % 4 != w) continue;
         float4v t = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (wt[i] != 0.f) t += so[i][dt][lane] * wt[i];
-        if (mine) *(float4v *)(a.part_o + part * D + 16 * dt + 4 * g) = t;
+        for (int i = 0; i < 4; ++i) t += sh.o[i][dt][lane] * wt[i];
+        if (mine) *(float4v *)(a.few_o + part * D + 16 * dt + 4 * g) = t;
     }
     if (mine && g == 0 && w == 0) {
-        a.part_ml[2 * part] = M;
-        a.part_ml[2 * part + 1] = l;
-    }
-}
-
-// One row's parts joined by a wave: nz parts, `step` parts apart.
-template <int D, bool BF>
-__device__ __forceinline__ void join_parts(const float *po, const float *ml, size_t first, size_t step, uint32_t nz,
-                                           uint16_t *out, float *lse) {
-    constexpr int V = D / 64;
-    const int lane = threadIdx.x & 63;
-    float M = -INFINITY;
-    for (uint32_t z = lane; z < nz; z += 64) M = fmaxf(M, ml[2 * (first + z * step)]);
-    M = wave_max(M);
-    float l = 0.f, o[V] = {};
-    for (uint32_t z = 0; z < nz; ++z) {
-        const size_t p = first + z * step;
-        const float mz = ml[2 * p], lz = ml[2 * p + 1];
-        const float wt = mz == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mz - M);
-        if (lz != lz) l = lz;
-        if (wt == 0.f) continue;
-        l += wt * lz;
-#pragma unroll
-        for (int i = 0; i < V; ++i) o[i] = fmaf(wt, po[p * D + V * lane + i], o[i]);
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    if constexpr (V == 2) {
-        *(uint32_t *)(out + 2 * lane) = l != l ? pack2<BF>(l, l) : pack2<BF>(o[0] * inv, o[1] * inv);
-    } else {
-        out[lane] = (uint16_t)(l != l ? pack2<BF>(l, l) : pack2<BF>(o[0] * inv, 0.f));
-    }
-    if (lse && lane == 0) *lse = l == 0.f ? -INFINITY : (M + __builtin_amdgcn_logf(l)) * LN2;
-}
-
-// Block = (sequence, KV head), its waves take the rows in turn.
-template <int D, bool BF>
-__global__ __launch_bounds__(256) void merge_few_kernel(AttnArgs a) {
-    const uint32_t hkv = a.b.hkv, kvh = blockIdx.x % hkv, s = blockIdx.x / hkv;
-    const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const PagedSeq sq = paged_seq(a.b, s);
-    const uint32_t n = paged_min(sq.n, a.b.max_q), R = n * a.G;
-    if (R == 0 || R > FEW) return;
-    const uint32_t prefix = a.prefix ? a.prefix[s] : 0u;
-    const uint32_t lo = paged_span(sq.first, sq.len, prefix, a.window).lo & ~31u;
-    const uint32_t hi = paged_span(sq.first + (int32_t)n - 1, sq.len, prefix, a.window).hi;
-    const uint32_t steps = hi > lo ? (hi - lo + 31) / 32 : 0;
-    if (steps <= a.chunk) return;
-    const uint32_t nz = (steps + a.chunk - 1) / a.chunk;
-    for (uint32_t r = w; r < R; r += 4) {
-        const size_t row = sq.row0 + r / a.G;
-        const uint32_t head = kvh * a.G + r % a.G;
-        join_parts<D, BF>(a.part_o, a.part_ml, (((size_t)s * hkv + kvh) * a.splits) * FEW + r, FEW, nz,
-                          a.out + row * a.o_stride + head * D, a.lse ? a.lse + row * a.hq + head : nullptr);
+        a.few_ml[2 * part] = M;
+        a.few_ml[2 * part + 1] = l;
     }
 }
 
@@ -408,31 +344,10 @@ __device__ __forceinline__ void load_to_lds(const void *sbase, uint32_t voff, ui
 
 // What unit u of the batch's row tiles is: tile `tile` of sequence `s`.
 __device__ __forceinline__ bool find_tile(const AttnArgs &a, uint32_t u, uint32_t *s, uint32_t *tile) {
-    const uint32_t lane = threadIdx.x & 63;
-    uint32_t before = 0;
-    for (uint32_t base = 0; base < a.b.num_seqs; base += 64) {
-        uint32_t cnt = 0;
-        if (base + lane < a.b.num_seqs) {
-            const uint32_t rows = paged_min(paged_seq(a.b, base + lane).n, a.b.max_q) * a.G;
-            cnt = rows <= a.few ? 0u : (rows + TILE_ROWS - 1) / TILE_ROWS;
-        }
-        uint32_t upto = cnt;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint32_t t = __shfl_up(upto, o);
-            upto += lane >= (uint32_t)o ? t : 0u;
-        }
-        const uint32_t all = __builtin_amdgcn_readlane(upto, 63);
-        if (u - before < all) {
-            const uint64_t in = __builtin_amdgcn_ballot_w64(u - before < upto);
-            const uint32_t i = __builtin_amdgcn_readfirstlane(__builtin_ctzll(in));
-            *s = base + i;
-            *tile = u - before - __builtin_amdgcn_readlane(upto - cnt, i);
-            return true;
-        }
-        before += all;
-    }
-    return false;
+    return paged_find(a.b.num_seqs, u, s, tile, [&](uint32_t i) {
+        const uint32_t rows = paged_min(paged_seq(a.b, i).n, a.b.max_q) * a.G;
+        return rows <= a.few ? 0u : (rows + TILE_ROWS - 1) / TILE_ROWS;
+    });
 }
 
 // Tile `tile` of sequence s: its rows and its keys, in tiles of KT.
@@ -451,7 +366,7 @@ __device__ __forceinline__ RowTile row_tile(const AttnArgs &a, uint32_t s, uint3
     t.hi = paged_span(t.sq.first + (int32_t)(last / a.G), t.sq.len, t.prefix, a.window).hi;
     t.t0 = t.lo / KT;
     t.t1 = t.hi > t.lo ? (t.hi + KT - 1) / KT : t.t0;
-    t.nz = a.splits > 1 && t.t1 - t.t0 > a.chunk ? (t.t1 - t.t0 + a.chunk - 1) / a.chunk : 1;
+    t.nz = a.chunk_splits > 1 && t.t1 - t.t0 > a.chunk_tiles ? (t.t1 - t.t0 + a.chunk_tiles - 1) / a.chunk_tiles : 1;
     return t;
 }
 
@@ -462,23 +377,27 @@ __device__ __forceinline__ RowTile row_tile(const AttnArgs &a, uint32_t s, uint3
 // LDS with their 16-byte pieces rotated (piece p of row r at slot p ^ r), V as
 // its pages have it, [16-key group][dim][16 keys], where a wave's operand is
 // one contiguous run.
+template <int D>
+struct ChunkShared {
+    uint16_t k[2][KT * D], v[2][KT * D];
+};
+
 template <int D, bool BF, bool GEN>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void chunk_kernel(AttnArgs a) {
+__device__ __forceinline__ void chunk_part(const AttnArgs &a, uint32_t block, ChunkShared<D> &sh) {
     constexpr int NKS = D / 16, NDT = D / 32, PIECES = D / 8;   // pieces of 16 bytes in a K row
     constexpr int TILE = KT * D, LOADS = TILE / 8 / 256;
-    __shared__ __align__(16) uint16_t Ks[2][TILE], Vs[2][TILE];
     const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5, c = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     // KV head fastest: with 8 of them each XCD keeps one head's K and V in its L2;
     // the last tiles, which see the most keys, first
-    const uint32_t hkv = a.b.hkv, kvh = blockIdx.x % hkv, z = blockIdx.x / hkv % a.splits;
-    const uint32_t u = a.units - 1 - blockIdx.x / hkv / a.splits;
+    const uint32_t hkv = a.b.hkv, kvh = block % hkv, z = block / hkv % a.chunk_splits;
+    const uint32_t u = a.units - 1 - block / hkv / a.chunk_splits;
     uint32_t s, tile;
     if (!find_tile(a, u, &s, &tile)) return;
     const RowTile rt = row_tile(a, s, tile);
     if (z >= rt.nz) return;
-    const uint32_t t0 = a.splits > 1 ? rt.t0 + z * a.chunk : rt.t0;
-    const uint32_t t1 = a.splits > 1 ? paged_min(rt.t1, t0 + a.chunk) : rt.t1;
+    const uint32_t t0 = a.chunk_splits > 1 ? rt.t0 + z * a.chunk_tiles : rt.t0;
+    const uint32_t t1 = a.chunk_splits > 1 ? paged_min(rt.t1, t0 + a.chunk_tiles) : rt.t1;
 
     const uint32_t w0 = rt.r0 + 32u * (uint32_t)wave;
     const bool any = w0 < rt.R;   // wave-uniform
@@ -504,15 +423,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void c
     auto pages_of = [&](uint32_t t) __attribute__((always_inline)) {
         Pages p;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) p.p[i] = page_at(a.b, s, t * KT + 16 * i, t < t1 && t * KT + 16 * i < rt.hi);
+        for (int i = 0; i < 4; ++i) p.p[i] = paged_entry(a.b, s, t * KT + 16 * i, t < t1 && t * KT + 16 * i < rt.hi);
         return p;
     };
     auto stage = [&](uint32_t t, const Pages &p) __attribute__((always_inline)) {
         const uint32_t k0 = t * KT, buf = t & 1;
         const uint32_t lk = __builtin_amdgcn_readfirstlane(
-            (uint32_t)(size_t)(__attribute__((address_space(3))) uint16_t *)(Ks[buf] + 8 * 64 * wave));
+            (uint32_t)(size_t)(__attribute__((address_space(3))) uint16_t *)(sh.k[buf] + 8 * 64 * wave));
         const uint32_t lv = __builtin_amdgcn_readfirstlane(
-            (uint32_t)(size_t)(__attribute__((address_space(3))) uint16_t *)(Vs[buf] + 8 * 64 * wave));
+            (uint32_t)(size_t)(__attribute__((address_space(3))) uint16_t *)(sh.v[buf] + 8 * 64 * wave));
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
             uint32_t page, in;
@@ -556,6 +475,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void c
         for (int e = 0; e < 16; ++e) o[dt][e] = 0.f;
     const float cs = GEN ? 1.f : a.scale, ahead = 8.f / cs;
     float m = -INFINITY, nm = 0.f, l = 0.f;
+    uint32_t odd = 0;
+    auto in_part = [&](uint32_t kk0, uint32_t gone) { return kk0 < last.lo || kk0 + 32 > first.hi || gone; };   // wave-uniform
     const int krm = (c & 19) | ((c & 4) << 1) | ((c & 8) >> 1);   // key of A row c
 
     for (uint32_t t = t0; t < t1; ++t) {
@@ -571,7 +492,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void c
             cur = next;
             next = pages_of(t + 2);
         }
-        const uint16_t *const Kt = Ks[t & 1], *const Vt = Vs[t & 1];
+        const uint16_t *const Kt = sh.k[t & 1], *const Vt = sh.v[t & 1];
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) {
             const uint32_t kk0 = t * KT + 32u * kt;
@@ -592,16 +513,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void c
                     sc[e] = general_score(a, sc[e], slope, pos - (int32_t)(key + 16 * (e >> 3) + (e & 7)));
             }
             const uint32_t gone = bad >> (2 * kt) & 3;
-            const bool masked = kk0 < last.lo || kk0 + 32 > first.hi || gone;   // wave-uniform
-            uint32_t vis = 0xFFFF;
+            const bool masked = in_part(kk0, gone);
             if (masked) {
-                vis = 0;
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     const uint32_t j = key + 16 * (e >> 3) + (e & 7);
-                    const bool on = j >= sp.lo && j < sp.hi && !(gone >> (e >> 3) & 1);
-                    vis |= (on ? 1u : 0u) << e;
-                    sc[e] = on ? sc[e] : -INFINITY;
+                    sc[e] = j >= sp.lo && j < sp.hi && !(gone >> (e >> 3) & 1) ? sc[e] : -INFINITY;
                 }
             }
             float mx = sc[0];
@@ -634,17 +551,30 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void c
                 const uint16_t *const vrow = Vt + (2 * kt + st) * (16 * D) + c * 16 + 8 * hh;
                 if (masked) {
 #pragma unroll
-                    for (int dt = 0; dt < NDT; ++dt) {
-                        const v4u v = *(const v4u *)(vrow + 32 * 16 * dt);
-                        if (__builtin_amdgcn_ballot_w64(nonfinite<BF>(v) != 0))   // wave-uniform, rare
-                            add_nonfinite<BF>(o[dt], v, p, vis >> (8 * st), mfma32<BF>);
-                        else
-                            o[dt] = mfma32<BF>(v, p, o[dt]);
-                    }
+                    for (int dt = 0; dt < NDT; ++dt)
+                        o[dt] = mfma32<BF>(finite_part<BF>(*(const v4u *)(vrow + 32 * 16 * dt), odd), p, o[dt]);
                 } else {
 #pragma unroll
                     for (int dt = 0; dt < NDT; ++dt) o[dt] = mfma32<BF>(*(const v4u *)(vrow + 32 * 16 * dt), p, o[dt]);
                 }
+            }
+        }
+    }
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(odd != 0) != 0, 0)) {   // wave-uniform
+        for (uint32_t kk0 = t0 * KT; kk0 < t1 * KT; kk0 += 32) {
+            const bool hole = paged_entry(a.b, s, kk0, kk0 < rt.hi) == a.b.num_pages ||
+                              paged_entry(a.b, s, kk0 + 16, kk0 + 16 < rt.hi) == a.b.num_pages;
+            if (!in_part(kk0, hole)) continue;   // whole steps had V as it is
+            for (uint32_t key = kk0; key < kk0 + 32; ++key) {
+                const uint32_t page = paged_entry(a.b, s, key, key < rt.hi);
+                if (page == a.b.num_pages) continue;
+                const uint16_t *vp = a.v + ((((size_t)page * hkv + kvh) * D) << a.b.shift) + (key & pmask);
+                const bool seen = key >= sp.lo && key < sp.hi;
+#pragma unroll
+                for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        o[dt][e] += odd_value<BF>(vp[(size_t)(32 * dt + 8 * (e >> 2) + 4 * hh + (e & 3)) << a.b.shift], seen);
             }
         }
     }
@@ -653,16 +583,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void c
     if (!any || w0 + (uint32_t)c >= rt.R) return;
     const float M = -nm;
     if (rt.nz > 1) {
-        const size_t part = (((size_t)u * hkv + kvh) * a.splits + z) * TILE_ROWS + (w0 - rt.r0) + (uint32_t)c;
+        const size_t part = (((size_t)u * hkv + kvh) * a.chunk_splits + z) * TILE_ROWS + (w0 - rt.r0) + (uint32_t)c;
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                *(float4v *)(a.part_o + part * D + 32 * dt + 8 * j + 4 * hh) =
+                *(float4v *)(a.chunk_o + part * D + 32 * dt + 8 * j + 4 * hh) =
                     (float4v){o[dt][4 * j], o[dt][4 * j + 1], o[dt][4 * j + 2], o[dt][4 * j + 3]};
         if (hh == 0) {
-            a.part_ml[2 * part] = m == -INFINITY ? -INFINITY : M;
-            a.part_ml[2 * part + 1] = l;
+            a.chunk_ml[2 * part] = m == -INFINITY ? -INFINITY : M;
+            a.chunk_ml[2 * part + 1] = l;
         }
         return;
     }
@@ -679,54 +609,130 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void c
         a.lse[(size_t)(rt.sq.row0 + tok) * a.hq + head] = l == 0.f ? -INFINITY : (M + __builtin_amdgcn_logf(l)) * LN2;
 }
 
-// Block = 16 rows of a row tile whose keys were split, its waves in turn.
+// One launch for a batch: few_part's blocks first (they wait for memory while
+// the chunks' compute).
+enum { FEW_ONLY, CHUNK_ONLY, BOTH };
+template <int D, bool BF, bool GEN, int KIND>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void attn_kernel(AttnArgs a) {
+    __shared__ __align__(16) union {
+        char none;
+        typename std::conditional<KIND != CHUNK_ONLY, FewShared<D>, char>::type few;
+        typename std::conditional<KIND != FEW_ONLY, ChunkShared<D>, char>::type chunk;
+    } sh;
+    if constexpr (KIND == FEW_ONLY) few_part<D, BF, GEN>(a, blockIdx.x, sh.few);
+    else if constexpr (KIND == CHUNK_ONLY) chunk_part<D, BF, GEN>(a, blockIdx.x, sh.chunk);
+    else if (blockIdx.x < a.few_blocks) few_part<D, BF, GEN>(a, blockIdx.x, sh.few);
+    else chunk_part<D, BF, GEN>(a, blockIdx.x - a.few_blocks, sh.chunk);
+}
+
+// ------------------------------------------------------------- parts joined
+// A row's nz parts, `step` parts apart from `first` on, by a block: the weights
+// once, then 256 / (D / 4) parts at a time, four dims a thread.
+constexpr uint32_t MOST_SPLITS = 256;
 template <int D, bool BF>
-__global__ __launch_bounds__(256) void merge_chunk_kernel(AttnArgs a) {
-    const uint32_t hkv = a.b.hkv, kvh = blockIdx.x % hkv, u = blockIdx.x / hkv;
-    const uint32_t w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+__device__ __forceinline__ void join_parts(const float *po, const float *ml, size_t first, size_t step, uint32_t nz,
+                                           uint16_t *out, float *lse) {
+    constexpr uint32_t LANES = D / 4, SETS = 256 / LANES;
+    __shared__ float wt[MOST_SPLITS], red[2][4];
+    __shared__ float4v part[SETS][LANES];
+    const uint32_t tid = threadIdx.x, w = tid >> 6;
+    const float2 f = tid < nz ? *(const float2 *)(ml + 2 * (first + tid * step)) : make_float2(-INFINITY, 0.f);
+    float M = wave_max(f.x);
+    if ((tid & 63) == 0) red[0][w] = M;
+    __syncthreads();
+    M = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+    const float mine = f.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(f.x - M);
+    wt[tid] = mine;
+    // a part without keys holds l = 0, one with NaN scores l = NaN, whatever its weight
+    const float l1 = wave_sum(f.y != f.y ? f.y : mine * f.y);
+    if ((tid & 63) == 0) red[1][w] = l1;
+    __syncthreads();
+    const float l = red[1][0] + red[1][1] + red[1][2] + red[1][3];
+    const uint32_t set = tid / LANES, d = tid % LANES;
+    float4v o = {0.f, 0.f, 0.f, 0.f};
+    const float *p = po + (first + set * step) * D + 4 * d;
+#pragma unroll 4
+    for (uint32_t z = set; z < nz; z += SETS, p += SETS * step * D) {
+        const float4v v = *(const float4v *)p;
+        o += v * wt[z];
+    }
+    part[set][d] = o;
+    __syncthreads();
+    if (set) return;
+#pragma unroll
+    for (uint32_t i = 1; i < SETS; ++i) o += part[i][d];
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    o *= inv;
+    if (l != l) o = (float4v){l, l, l, l};
+    *(uint2 *)(out + 4 * d) = make_uint2(pack2<BF>(o[0], o[1]), pack2<BF>(o[2], o[3]));
+    if (lse && d == 0) *lse = l == 0.f ? -INFINITY : (M + __builtin_amdgcn_logf(l)) * LN2;
+}
+
+// Block = a row: of (sequence, KV head) for few_part's, of (row tile, KV head)
+// for chunk_part's, which come after.
+template <int D, bool BF>
+__global__ __launch_bounds__(256) void join_kernel(AttnArgs a, uint32_t few_rows_blocks) {
+    const uint32_t hkv = a.b.hkv;
+    if (blockIdx.x < few_rows_blocks) {
+        const uint32_t r = blockIdx.x % a.few_rows, unit = blockIdx.x / a.few_rows, kvh = unit % hkv, s = unit / hkv;
+        const PagedSeq sq = paged_seq(a.b, s);
+        const uint32_t n = paged_min(sq.n, a.b.max_q), R = n * a.G;
+        if (r >= R || R > FEW) return;
+        const uint32_t prefix = a.prefix ? a.prefix[s] : 0u;
+        const uint32_t lo = paged_span(sq.first, sq.len, prefix, a.window).lo & ~31u;
+        const uint32_t hi = paged_span(sq.first + (int32_t)n - 1, sq.len, prefix, a.window).hi;
+        const uint32_t steps = hi > lo ? (hi - lo + 31) / 32 : 0;
+        if (steps <= a.few_steps) return;
+        const size_t row = sq.row0 + r / a.G;
+        const uint32_t head = kvh * a.G + r % a.G;
+        join_parts<D, BF>(a.few_o, a.few_ml, (size_t)unit * a.few_splits * a.few_rows + r, a.few_rows,
+                          (steps + a.few_steps - 1) / a.few_steps, a.out + row * a.o_stride + head * D,
+                          a.lse ? a.lse + row * a.hq + head : nullptr);
+        return;
+    }
+    const uint32_t block = blockIdx.x - few_rows_blocks, r = block % TILE_ROWS, unit = block / TILE_ROWS;
+    const uint32_t kvh = unit % hkv, u = unit / hkv;
     uint32_t s, tile;
     if (!find_tile(a, u, &s, &tile)) return;
     const RowTile rt = row_tile(a, s, tile);
-    if (rt.nz == 1) return;
-    for (uint32_t i = w; i < 16; i += 4) {
-        const uint32_t r = blockIdx.y * 16 + i;
-        if (rt.r0 + r >= rt.R) return;
-        const size_t row = rt.sq.row0 + (rt.r0 + r) / a.G;
-        const uint32_t head = kvh * a.G + (rt.r0 + r) % a.G;
-        join_parts<D, BF>(a.part_o, a.part_ml, ((size_t)u * hkv + kvh) * a.splits * TILE_ROWS + r, TILE_ROWS, rt.nz,
-                          a.out + row * a.o_stride + head * D, a.lse ? a.lse + row * a.hq + head : nullptr);
-    }
+    if (rt.nz == 1 || rt.r0 + r >= rt.R) return;
+    const size_t row = rt.sq.row0 + (rt.r0 + r) / a.G;
+    const uint32_t head = kvh * a.G + (rt.r0 + r) % a.G;
+    join_parts<D, BF>(a.chunk_o, a.chunk_ml, (size_t)unit * a.chunk_splits * TILE_ROWS + r, TILE_ROWS, rt.nz,
+                      a.out + row * a.o_stride + head * D, a.lse ? a.lse + row * a.hq + head : nullptr);
 }
 
 // ------------------------------------------------------------------- launch
-// Which kernels run and how keys are split, from the host's bounds alone.
+// Which parts run and how keys are split, from the host's bounds alone.
 struct Plan {
-    uint32_t few_splits = 0, few_chunk = 0;                // 0 splits: not launched
+    uint32_t few_rows = 0, few_splits = 0, few_steps = 0;          // 0 splits: not launched
     uint32_t units = 0, chunk_splits = 0, chunk_tiles = 0;
-    size_t few_parts = 0, chunk_parts = 0;                 // rows of partial results
+    size_t few_parts = 0, chunk_parts = 0;                         // rows of partial results
 };
 
 Plan plan_of(const nnz_paged_kv &kv, const nnz_paged_batch &b, uint32_t hq) {
     Plan p;
     const uint32_t G = hq / kv.num_kv_heads, hkv = kv.num_kv_heads;
     const uint64_t most = (uint64_t)b.max_q_len * G;   // rows of a sequence
-    // One sequence whose bound passes 16 rows goes to the chunk kernel, whatever
-    // its length turns out to be; a batch of several may hold both kinds.
-    if (G <= FEW && (most <= FEW || b.num_seqs > 1)) {
-        const uint32_t steps = (b.max_kv_len + 31) / 32, blocks = b.num_seqs * hkv;
-        const uint32_t want = std::max(1u, 2048 / blocks), most_splits = std::max(1u, steps / 16);
-        const uint32_t splits = std::min(want, most_splits);
-        p.few_chunk = (steps + splits - 1) / splits;
-        p.few_splits = (steps + p.few_chunk - 1) / p.few_chunk;
-        if (p.few_splits > 1) p.few_parts = (size_t)blocks * p.few_splits * FEW;
+    const bool chunks = most > FEW;
+    // One sequence whose bound passes 16 rows goes to chunk_part, whatever its
+    // length turns out to be; a batch of several may hold both kinds.
+    if (G <= FEW && (!chunks || b.num_seqs > 1)) {
+        const uint32_t steps = (b.max_kv_len + 31) / 32, blocks = b.num_seqs * hkv;   // below 2^26
+        const uint32_t want = std::max(1u, (chunks ? 512u : 1024u) / blocks), most_splits = std::max(1u, steps / 16);
+        const uint32_t splits = std::min({want, most_splits, MOST_SPLITS});
+        p.few_rows = (uint32_t)std::min<uint64_t>(most, FEW);
+        p.few_steps = (steps + splits - 1) / splits;
+        p.few_splits = (steps + p.few_steps - 1) / p.few_steps;
+        if (p.few_splits > 1) p.few_parts = (size_t)blocks * p.few_splits * p.few_rows;
     }
-    if (most > FEW || G > FEW) {
+    if (chunks) {
         const uint64_t by_rows = (uint64_t)b.num_rows * G / TILE_ROWS + b.num_seqs;
         const uint64_t by_seqs = (uint64_t)b.num_seqs * ((most + TILE_ROWS - 1) / TILE_ROWS);
         p.units = (uint32_t)std::min(by_rows, by_seqs);
         const uint32_t tiles = (b.max_kv_len + KT - 1) / KT;
-        const uint32_t want = std::max(1u, 512 / (p.units * hkv)), most_splits = std::max(1u, tiles / 4);
-        const uint32_t splits = std::min(want, most_splits);
+        const uint32_t want = (uint32_t)std::max<uint64_t>(1, 512 / ((uint64_t)p.units * hkv)), most_splits = std::max(1u, tiles / 4);
+        const uint32_t splits = std::min({want, most_splits, MOST_SPLITS});
         p.chunk_tiles = (tiles + splits - 1) / splits;
         p.chunk_splits = (tiles + p.chunk_tiles - 1) / p.chunk_tiles;
         if (p.chunk_splits > 1) p.chunk_parts = (size_t)p.units * hkv * p.chunk_splits * TILE_ROWS;
@@ -734,28 +740,33 @@ Plan plan_of(const nnz_paged_kv &kv, const nnz_paged_batch &b, uint32_t hq) {
     return p;
 }
 
+uint64_t blocks_of(const Plan &p, const nnz_paged_batch &b, uint32_t hkv) {
+    return (uint64_t)b.num_seqs * hkv * p.few_splits + (uint64_t)p.units * hkv * p.chunk_splits;
+}
 size_t bytes_of(const Plan &p, uint32_t head_dim) { return (p.few_parts + p.chunk_parts) * (head_dim + 2) * 4; }
 
 template <int D, bool BF, bool GEN>
 void start(hipStream_t stream, const Plan &p, AttnArgs a, float *ws) {
     const uint32_t hkv = a.b.hkv;
-    if (p.chunk_splits) {
-        a.units = p.units;
-        a.splits = p.chunk_splits;
-        a.chunk = p.chunk_tiles;
-        a.part_o = ws;
-        a.part_ml = ws + p.chunk_parts * D;
-        chunk_kernel<D, BF, GEN><<<p.units * hkv * p.chunk_splits, 256, 0, stream>>>(a);
-        if (p.chunk_splits > 1) merge_chunk_kernel<D, BF><<<dim3(p.units * hkv, TILE_ROWS / 16), 256, 0, stream>>>(a);
-    }
-    if (p.few_splits) {
-        a.splits = p.few_splits;
-        a.chunk = p.few_chunk;
-        a.part_o = ws + p.chunk_parts * (D + 2);
-        a.part_ml = a.part_o + p.few_parts * D;
-        few_kernel<D, BF, GEN><<<a.b.num_seqs * hkv * p.few_splits, 256, 0, stream>>>(a);
-        if (p.few_splits > 1) merge_few_kernel<D, BF><<<a.b.num_seqs * hkv, 256, 0, stream>>>(a);
-    }
+    a.few = p.few_splits ? FEW : 0;
+    a.few_rows = p.few_rows;
+    a.few_splits = p.few_splits;
+    a.few_steps = p.few_steps;
+    a.few_blocks = a.b.num_seqs * hkv * p.few_splits;
+    a.units = p.units;
+    a.chunk_splits = p.chunk_splits;
+    a.chunk_tiles = p.chunk_tiles;
+    a.few_o = ws;
+    a.few_ml = a.few_o + p.few_parts * D;
+    a.chunk_o = a.few_ml + p.few_parts * 2;
+    a.chunk_ml = a.chunk_o + p.chunk_parts * D;
+    const uint32_t chunk_blocks = p.units * hkv * p.chunk_splits;
+    if (!chunk_blocks) attn_kernel<D, BF, GEN, FEW_ONLY><<<a.few_blocks, 256, 0, stream>>>(a);
+    else if (!a.few_blocks) attn_kernel<D, BF, GEN, CHUNK_ONLY><<<chunk_blocks, 256, 0, stream>>>(a);
+    else attn_kernel<D, BF, GEN, BOTH><<<a.few_blocks + chunk_blocks, 256, 0, stream>>>(a);
+    const uint32_t few_join = p.few_parts ? a.b.num_seqs * hkv * p.few_rows : 0;
+    const uint32_t chunk_join = p.chunk_parts ? p.units * hkv * TILE_ROWS : 0;
+    if (few_join + chunk_join) join_kernel<D, BF><<<few_join + chunk_join, 256, 0, stream>>>(a, few_join);
 }
 
 template <int D, bool BF>
@@ -780,6 +791,8 @@ extern "C" int nnz_dispatch_paged_attention(nnz_ctx *ctx, const nnz_paged_kv *kv
         return nnz_fail(ctx, f.code, "paged_attention: %s", f.what);
     const Plan plan = plan_of(*kv, *batch, p->num_query_heads);
     const size_t need = bytes_of(plan, kv->head_dim);
+    NNZ_REQUIRE(ctx, blocks_of(plan, *batch, kv->num_kv_heads) < (1u << 24), NNZ_EUNSUPPORTED,
+                "paged_attention: more than 2^24 blocks; split the batch");
     NNZ_REQUIRE(ctx, need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0), NNZ_EINVAL,
                 "paged_attention: workspace of %zu bytes, 16-byte aligned, needed (%zu given)", need, workspace_bytes);
     NnzDeviceScope scope(ctx);
@@ -801,7 +814,6 @@ extern "C" int nnz_dispatch_paged_attention(nnz_ctx *ctx, const nnz_paged_kv *kv
     a.scale = scale * LOG2E;
     a.cap = p->softcap * LOG2E;
     a.cap_in = p->softcap > 0.f ? 2.f * LOG2E * scale / p->softcap : 0.f;
-    a.few = plan.few_splits ? FEW : 0;
     const bool bf = kv->dtype == NNZ_BF16;
     float *ws = (float *)workspace;
     if (kv->head_dim == 128) bf ? start_scores<128, true>(ctx->stream, plan, a, ws) : start_scores<128, false>(ctx->stream, plan, a, ws);

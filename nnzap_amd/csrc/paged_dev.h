@@ -52,3 +52,40 @@ __device__ __forceinline__ float2 paged_cos_sin(int32_t p, const double *inv_fre
     sincospif(2.f * (float)(t - rint(t)), &s, &c);
     return make_float2(c, s);
 }
+
+// A table entry through the scalar cache (the table does not change while the
+// kernel runs); num_pages where there is no page or the keys are not wanted.
+__device__ __forceinline__ uint32_t paged_entry(const PagedView &b, uint32_t s, uint32_t key, bool wanted) {
+    const uint32_t e = key >> b.shift;
+    if (!wanted || e >= b.width) return b.num_pages;
+    typedef const uint32_t __attribute__((address_space(4))) *table_t;
+    const table_t t = (table_t)(uintptr_t)(b.table + (size_t)s * b.width);
+    return paged_min(t[e], b.num_pages);
+}
+
+// Unit u of a batch whose sequence i has count(i) units: which sequence's, and
+// which of its units.  By whole waves, 64 sequences at a time.
+template <class Count>
+__device__ __forceinline__ bool paged_find(uint32_t num_seqs, uint32_t u, uint32_t *s, uint32_t *unit, Count count) {
+    const uint32_t lane = threadIdx.x & 63;
+    uint32_t before = 0;
+    for (uint32_t base = 0; base < num_seqs; base += 64) {
+        const uint32_t cnt = base + lane < num_seqs ? count(base + lane) : 0u;
+        uint32_t upto = cnt;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t t = __shfl_up(upto, o);
+            upto += lane >= (uint32_t)o ? t : 0u;
+        }
+        const uint32_t all = __builtin_amdgcn_readlane(upto, 63);
+        if (u - before < all) {
+            const uint64_t in = __builtin_amdgcn_ballot_w64(u - before < upto);
+            const uint32_t i = __builtin_amdgcn_readfirstlane(__builtin_ctzll(in));
+            *s = base + i;
+            *unit = u - before - __builtin_amdgcn_readlane(upto - cnt, i);
+            return true;
+        }
+        before += all;
+    }
+    return false;
+}
