@@ -165,22 +165,24 @@ __device__ __forceinline__ void few_part(const AttnArgs &a, uint32_t block, FewS
         for (int ks = 0; ks < NKS; ++ks) qf[ks] = *(const v4u *)(qp + 32 * ks + 8 * g);
     }
 
-    const uint32_t pmask = (1u << a.b.shift) - 1;
+    // elements of a page; this head's part of page 0
+    const uint32_t pmask = (1u << a.b.shift) - 1, page_len = (hkv * D) << a.b.shift;
+    const uint16_t *const kh = a.k + (((size_t)kvh * D) << a.b.shift), *const vh = a.v + (((size_t)kvh * D) << a.b.shift);
     auto load = [&](FewStep<D, BF> &f, uint32_t st) __attribute__((always_inline)) {
         const uint32_t k0 = lo + 32 * st;
-        uint32_t pa = paged_entry(a.b, s, k0, true), pb = paged_entry(a.b, s, k0 + 16, k0 + 16 < hi);
-        f.bad = (pa == a.b.num_pages ? 1u : 0u) | (pb == a.b.num_pages ? 2u : 0u);
+        uint32_t pa = paged_raw(a.b, s, k0), pb = paged_raw(a.b, s, k0 + 16);
+        f.bad = (pa < a.b.num_pages ? 0u : 1u) | (k0 + 16 < hi && pb < a.b.num_pages ? 0u : 2u);
         pa = f.bad & 1 ? 0u : pa;   // any page: the keys are masked
         pb = f.bad & 2 ? 0u : pb;
-        const size_t ha = (size_t)pa * hkv + kvh, hb = (size_t)pb * hkv + kvh;
+        const uint64_t ha = (uint64_t)pa * page_len, hb = (uint64_t)pb * page_len;
         const uint32_t oa = k0 & pmask, ob = (k0 + 16) & pmask;
-        const uint16_t *ka = a.k + ((ha << a.b.shift) + oa) * D, *kb = a.k + ((hb << a.b.shift) + ob) * D;
+        const uint16_t *ka = kh + ha + oa * D, *kb = kh + hb + ob * D;
         const uint16_t *kp = (c < 8 ? ka : kb) + (8 * (c >> 2 & 1) + (c & 3)) * D + 8 * g;
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int ks = 0; ks < NKS; ++ks) f.k[i][ks] = *(const v4u *)(kp + 4 * i * D + 32 * ks);
-        const uint16_t *va = a.v + ((ha * D) << a.b.shift) + oa, *vb = a.v + ((hb * D) << a.b.shift) + ob;
+        const uint16_t *va = vh + ha + oa, *vb = vh + hb + ob;
         const uint16_t *vp = (g < 2 ? va : vb) + ((size_t)c << a.b.shift) + 8 * (g & 1);
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt) f.v[dt] = *(const v4u *)(vp + ((size_t)(16 * dt) << a.b.shift));
@@ -271,7 +273,7 @@ __device__ __forceinline__ void few_part(const AttnArgs &a, uint32_t block, FewS
             for (uint32_t key = k0; key < k0 + 32; ++key) {
                 const uint32_t page = paged_entry(a.b, s, key, key < hi);
                 if (page == a.b.num_pages) continue;
-                const uint16_t *vp = a.v + ((((size_t)page * hkv + kvh) * D) << a.b.shift) + (key & pmask);
+                const uint16_t *vp = vh + (uint64_t)page * page_len + (key & pmask);
                 const bool seen = key >= sp.lo && key < sp.hi;
 #pragma unroll
                 for (int dt = 0; dt < NDT; ++dt)
@@ -299,8 +301,7 @@ __device__ __forceinline__ void few_part(const AttnArgs &a, uint32_t block, FewS
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         wt[i] = sh.m[i][c] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sh.m[i][c] - M);
-        l += wt[i] * sh.l[i][c];
-        if (sh.l[i][c] != sh.l[i][c]) l = sh.l[i][c];
+        l += wt[i] * sh.l[i][c];   // NaN stays NaN, times 0 too
     }
     const bool mine = (uint32_t)c < R;
     if (nz == 1) {
@@ -312,7 +313,6 @@ __device__ __forceinline__ void few_part(const AttnArgs &a, uint32_t block, FewS
             float4v t = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < 4; ++i) t += sh.o[i][dt][lane] * wt[i];
-            if (l != l) t = (float4v){l, l, l, l};
             if (mine)
                 *(uint2 *)(op + 16 * dt) = make_uint2(pack2<BF>(t[0] * inv, t[1] * inv), pack2<BF>(t[2] * inv, t[3] * inv));
         }
@@ -416,16 +416,19 @@ __device__ __forceinline__ void chunk_part(const AttnArgs &a, uint32_t block, Ch
     const uint32_t krow = (uint32_t)lane / PIECES + (uint32_t)wave * RPW;
     const uint32_t koff = ((krow & 15) * D + 8 * (((uint32_t)lane % PIECES) ^ (krow & (PIECES - 1)))) * 2u;
     const uint32_t vp = ((uint32_t)tid) % (2 * D), voff = ((vp / 2) << a.b.shift) * 2u + (vp & 1) * 16u;
-    const uint32_t pmask = (1u << a.b.shift) - 1;
+    // elements of a page; this head's part of page 0
+    const uint32_t pmask = (1u << a.b.shift) - 1, page_len = (hkv * D) << a.b.shift;
+    const uint16_t *const kh = a.k + (((size_t)kvh * D) << a.b.shift), *const vh = a.v + (((size_t)kvh * D) << a.b.shift);
     struct Pages {
-        uint32_t p[4];
+        uint32_t p[4];   // table entries of the tile's groups of 16 keys, as they stand there
     };
     auto pages_of = [&](uint32_t t) __attribute__((always_inline)) {
         Pages p;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) p.p[i] = paged_entry(a.b, s, t * KT + 16 * i, t < t1 && t * KT + 16 * i < rt.hi);
+        for (int i = 0; i < 4; ++i) p.p[i] = paged_raw(a.b, s, t * KT + 16 * i);
         return p;
     };
+    auto has_page = [&](const Pages &p, uint32_t t, int i) { return t * KT + 16 * i < rt.hi && p.p[i] < a.b.num_pages; };
     auto stage = [&](uint32_t t, const Pages &p) __attribute__((always_inline)) {
         const uint32_t k0 = t * KT, buf = t & 1;
         const uint32_t lk = __builtin_amdgcn_readfirstlane(
@@ -434,25 +437,25 @@ __device__ __forceinline__ void chunk_part(const AttnArgs &a, uint32_t block, Ch
             (uint32_t)(size_t)(__attribute__((address_space(3))) uint16_t *)(sh.v[buf] + 8 * 64 * wave));
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
-            uint32_t page, in;
+            uint32_t page, in;   // any page where there is none: the keys are masked
             if constexpr (D == 128) {
-                page = p.p[i];
+                page = has_page(p, t, i) ? p.p[i] : 0u;
                 in = 16 * i;
             } else {   // a piece index spans two groups
-                page = wave < 2 ? p.p[2 * i] : p.p[2 * i + 1];
+                const uint32_t lower = has_page(p, t, 2 * i) ? p.p[2 * i] : 0u, upper = has_page(p, t, 2 * i + 1) ? p.p[2 * i + 1] : 0u;
+                page = wave < 2 ? lower : upper;
                 in = 32 * i + (wave < 2 ? 0 : 16);
             }
-            page = page == a.b.num_pages ? 0u : page;   // any page: the keys are masked
-            const size_t h = (size_t)page * hkv + kvh;
+            const uint64_t at = (uint64_t)page * page_len;
             const uint32_t slot = (k0 + in) & pmask;
-            load_to_lds(a.k + ((h << a.b.shift) + slot) * D, koff, lk + 16u * (uint32_t)(i * 256));
-            load_to_lds(a.v + ((h * D) << a.b.shift) + slot, voff, lv + 16u * (uint32_t)(i * 256));
+            load_to_lds(kh + at + slot * D, koff, lk + 16u * (uint32_t)(i * 256));
+            load_to_lds(vh + at + slot, voff, lv + 16u * (uint32_t)(i * 256));
         }
     };
-    auto bad_of = [&](const Pages &p) __attribute__((always_inline)) {
+    auto bad_of = [&](const Pages &p, uint32_t t) __attribute__((always_inline)) {
         uint32_t bad = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) bad |= (p.p[i] == a.b.num_pages ? 1u : 0u) << i;
+        for (int i = 0; i < 4; ++i) bad |= (has_page(p, t, i) ? 0u : 1u) << i;
         return bad;
     };
 
@@ -476,7 +479,7 @@ __device__ __forceinline__ void chunk_part(const AttnArgs &a, uint32_t block, Ch
     const float cs = GEN ? 1.f : a.scale, ahead = 8.f / cs;
     float m = -INFINITY, nm = 0.f, l = 0.f;
     uint32_t odd = 0;
-    auto in_part = [&](uint32_t kk0, uint32_t gone) { return kk0 < last.lo || kk0 + 32 > first.hi || gone; };   // wave-uniform
+    auto in_part = [&](uint32_t k0, uint32_t gone) { return k0 < last.lo || k0 + KT > first.hi || gone; };   // wave-uniform
     const int krm = (c & 19) | ((c & 4) << 1) | ((c & 8) >> 1);   // key of A row c
 
     for (uint32_t t = t0; t < t1; ++t) {
@@ -486,89 +489,102 @@ __device__ __forceinline__ void chunk_part(const AttnArgs &a, uint32_t block, Ch
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        const uint32_t bad = bad_of(cur);
+        const uint32_t bad = bad_of(cur, t);
         if (t + 1 < t1) {   // block-uniform
             stage(t + 1, next);
             cur = next;
             next = pages_of(t + 2);
         }
         const uint16_t *const Kt = sh.k[t & 1], *const Vt = sh.v[t & 1];
+        const uint32_t k0 = t * KT;
+        if (!any || k0 >= last.hi || k0 + KT <= first.lo) continue;   // wave-uniform
+        // scores of both halves of the tile; the operands of a half are all read
+        // before its products, the second half's during the first one's
+        float16v sc[2];
+        v4u kf[2][NKS];
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) {
-            const uint32_t kk0 = t * KT + 32u * kt;
-            if (!any || kk0 >= last.hi || kk0 + 32 <= first.lo) continue;   // wave-uniform
             const int row = 32 * kt + krm;
-            float16v sc;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) sc[e] = 0.f;
+            for (int ks = 0; ks < NKS; ++ks)
+                kf[kt][ks] = *(const v4u *)(Kt + row * D + 8 * ((2 * ks + hh) ^ (row & (PIECES - 1))));
+            __builtin_amdgcn_sched_barrier(0);
+        }
 #pragma unroll
-            for (int ks = 0; ks < NKS; ++ks) {
-                const v4u kf = *(const v4u *)(Kt + row * D + 8 * ((2 * ks + hh) ^ (row & (PIECES - 1))));
-                sc = mfma32<BF>(kf, qf[ks], sc);
+        for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) sc[kt][e] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < NKS; ++ks) sc[kt] = mfma32<BF>(kf[kt][ks], qf[ks], sc[kt]);
+        }
+        // V^T of the first 16 keys, read while the softmax runs
+        v4u vf[NDT];
+        auto read_v = [&](int st) __attribute__((always_inline)) {
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt) vf[dt] = *(const v4u *)(Vt + st * (16 * D) + (32 * dt + c) * 16 + 8 * hh);
+        };
+        read_v(0);
+        __builtin_amdgcn_sched_barrier(0);
+        const uint32_t key = k0 + 8 * hh;   // register e of half kt: key + 32 kt + 16 (e >> 3) + (e & 7)
+        if constexpr (GEN) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+                sc[e >> 4][e & 15] = general_score(a, sc[e >> 4][e & 15], slope, pos - (int32_t)(key + 16 * (e >> 3) + (e & 7)));
+        }
+        const bool masked = in_part(k0, bad);
+        if (masked) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+                const uint32_t j = key + 16 * (e >> 3) + (e & 7);
+                const bool on = j >= sp.lo && j < sp.hi && !(bad >> (e >> 3) & 1);
+                sc[e >> 4][e & 15] = on ? sc[e >> 4][e & 15] : -INFINITY;
             }
-            const uint32_t key = kk0 + 8 * hh;   // register e: key + 16 (e >> 3) + (e & 7)
-            if constexpr (GEN) {
+        }
+        float mx = sc[0][0];
 #pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    sc[e] = general_score(a, sc[e], slope, pos - (int32_t)(key + 16 * (e >> 3) + (e & 7)));
+        for (int e = 1; e < 32; ++e) mx = fmaxf(mx, sc[e >> 4][e & 15]);
+        if (__builtin_amdgcn_ballot_w64(mx > m + ahead)) {   // wave-uniform
+            const float2 both = swap32(mx, mx);
+            mx = fmaxf(both.x, both.y);
+            const bool move = mx > m + ahead;
+            const float nm2 = move ? -mx * cs : nm;
+            const float alpha = move && m != -INFINITY ? __builtin_amdgcn_exp2f(nm2 - nm) : 1.f;
+            m = move ? mx : m;
+            nm = nm2;
+            l *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[dt][e] *= alpha;
+        }
+#pragma unroll
+        for (int st = 0; st < 4; ++st) {   // 16 keys each
+            v4u p;
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                const float x = __builtin_amdgcn_exp2f(fmaf(sc[st >> 1][8 * (st & 1) + e], cs, nm));
+                const float y = __builtin_amdgcn_exp2f(fmaf(sc[st >> 1][8 * (st & 1) + e + 1], cs, nm));
+                l += x;
+                l += y;
+                p[e / 2] = pack2<BF>(x, y);
             }
-            const uint32_t gone = bad >> (2 * kt) & 3;
-            const bool masked = in_part(kk0, gone);
             if (masked) {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const uint32_t j = key + 16 * (e >> 3) + (e & 7);
-                    sc[e] = j >= sp.lo && j < sp.hi && !(gone >> (e >> 3) & 1) ? sc[e] : -INFINITY;
-                }
-            }
-            float mx = sc[0];
-#pragma unroll
-            for (int e = 1; e < 16; ++e) mx = fmaxf(mx, sc[e]);
-            if (__builtin_amdgcn_ballot_w64(mx > m + ahead)) {   // wave-uniform
-                const float2 both = swap32(mx, mx);
-                mx = fmaxf(both.x, both.y);
-                const bool move = mx > m + ahead;
-                const float nm2 = move ? -mx * cs : nm;
-                const float alpha = move && m != -INFINITY ? __builtin_amdgcn_exp2f(nm2 - nm) : 1.f;
-                m = move ? mx : m;
-                nm = nm2;
-                l *= alpha;
-#pragma unroll
-                for (int dt = 0; dt < NDT; ++dt)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) o[dt][e] *= alpha;
+                for (int dt = 0; dt < NDT; ++dt) vf[dt] = finite_part<BF>(vf[dt], odd);
             }
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                sc[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], cs, nm));
-                l += sc[e];
-            }
-#pragma unroll
-            for (int st = 0; st < 2; ++st) {   // 16 keys each
-                v4u p;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) p[i] = pack2<BF>(sc[8 * st + 2 * i], sc[8 * st + 2 * i + 1]);
-                const uint16_t *const vrow = Vt + (2 * kt + st) * (16 * D) + c * 16 + 8 * hh;
-                if (masked) {
-#pragma unroll
-                    for (int dt = 0; dt < NDT; ++dt)
-                        o[dt] = mfma32<BF>(finite_part<BF>(*(const v4u *)(vrow + 32 * 16 * dt), odd), p, o[dt]);
-                } else {
-#pragma unroll
-                    for (int dt = 0; dt < NDT; ++dt) o[dt] = mfma32<BF>(*(const v4u *)(vrow + 32 * 16 * dt), p, o[dt]);
-                }
-            }
+            for (int dt = 0; dt < NDT; ++dt) o[dt] = mfma32<BF>(vf[dt], p, o[dt]);
+            if (st < 3) read_v(st + 1);
         }
     }
     if (__builtin_expect(__builtin_amdgcn_ballot_w64(odd != 0) != 0, 0)) {   // wave-uniform
-        for (uint32_t kk0 = t0 * KT; kk0 < t1 * KT; kk0 += 32) {
-            const bool hole = paged_entry(a.b, s, kk0, kk0 < rt.hi) == a.b.num_pages ||
-                              paged_entry(a.b, s, kk0 + 16, kk0 + 16 < rt.hi) == a.b.num_pages;
-            if (!in_part(kk0, hole)) continue;   // whole steps had V as it is
-            for (uint32_t key = kk0; key < kk0 + 32; ++key) {
+        for (uint32_t t = t0; t < t1; ++t) {
+            const uint32_t k0 = t * KT;
+            if (!in_part(k0, bad_of(pages_of(t), t))) continue;   // whole tiles had V as it is
+            for (uint32_t key = k0; key < k0 + KT; ++key) {
                 const uint32_t page = paged_entry(a.b, s, key, key < rt.hi);
                 if (page == a.b.num_pages) continue;
-                const uint16_t *vp = a.v + ((((size_t)page * hkv + kvh) * D) << a.b.shift) + (key & pmask);
+                const uint16_t *vp = vh + (uint64_t)page * page_len + (key & pmask);
                 const bool seen = key >= sp.lo && key < sp.hi;
 #pragma unroll
                 for (int dt = 0; dt < NDT; ++dt)
@@ -626,80 +642,114 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void a
 }
 
 // ------------------------------------------------------------- parts joined
-// A row's nz parts, `step` parts apart from `first` on, by a block: the weights
-// once, then 256 / (D / 4) parts at a time, four dims a thread.
+// A row takes D/4 threads (four dims each) times 1, 2, 4 or 8 sets that share
+// its parts out; a block holds as many rows as fit.  few_part's rows first, by
+// (sequence, KV head, row), then chunk_part's, by (row tile, KV head, row).
 constexpr uint32_t MOST_SPLITS = 256;
+struct JoinArgs {
+    uint64_t few_rows;            // rows of few_part's, rounded up to whole blocks
+    uint32_t few_sets, chunk_sets;
+};
+
+// The parts first + z step, z = set, set + sets, ..., then the sets' sums.
 template <int D, bool BF>
 __device__ __forceinline__ void join_parts(const float *po, const float *ml, size_t first, size_t step, uint32_t nz,
-                                           uint16_t *out, float *lse) {
-    constexpr uint32_t LANES = D / 4, SETS = 256 / LANES;
-    __shared__ float wt[MOST_SPLITS], red[2][4];
-    __shared__ float4v part[SETS][LANES];
-    const uint32_t tid = threadIdx.x, w = tid >> 6;
-    const float2 f = tid < nz ? *(const float2 *)(ml + 2 * (first + tid * step)) : make_float2(-INFINITY, 0.f);
-    float M = wave_max(f.x);
-    if ((tid & 63) == 0) red[0][w] = M;
-    __syncthreads();
-    M = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-    const float mine = f.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(f.x - M);
-    wt[tid] = mine;
-    // a part without keys holds l = 0, one with NaN scores l = NaN, whatever its weight
-    const float l1 = wave_sum(f.y != f.y ? f.y : mine * f.y);
-    if ((tid & 63) == 0) red[1][w] = l1;
-    __syncthreads();
-    const float l = red[1][0] + red[1][1] + red[1][2] + red[1][3];
-    const uint32_t set = tid / LANES, d = tid % LANES;
+                                           uint32_t sets, bool mine, uint16_t *out, float *lse) {
+    constexpr uint32_t LANES = D / 4;
+    __shared__ float4v part[256];
+    __shared__ float2 stat[256 / LANES];
+    const uint32_t tid = threadIdx.x, d = tid % LANES, team = tid / LANES, set = team % sets;
+    float M = -INFINITY, l = 0.f;
     float4v o = {0.f, 0.f, 0.f, 0.f};
-    const float *p = po + (first + set * step) * D + 4 * d;
-#pragma unroll 4
-    for (uint32_t z = set; z < nz; z += SETS, p += SETS * step * D) {
-        const float4v v = *(const float4v *)p;
-        o += v * wt[z];
-    }
-    part[set][d] = o;
-    __syncthreads();
-    if (set) return;
+    auto add = [&](float m2, float l2, float4v o2) {
+        const float to = fmaxf(M, m2);
+        const float f = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - to);
+        const float f2 = m2 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m2 - to);
+        M = to;
+        l = l * f + l2 * f2;
+        o = o * f + o2 * f2;
+    };
+    constexpr uint32_t AHEAD = 4;   // parts whose loads are in flight together
+    if (mine) {
+        for (uint32_t z0 = set; z0 < nz; z0 += AHEAD * sets) {
+            float2 f[AHEAD];
+            float4v v[AHEAD];
 #pragma unroll
-    for (uint32_t i = 1; i < SETS; ++i) o += part[i][d];
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    o *= inv;
-    if (l != l) o = (float4v){l, l, l, l};
+            for (uint32_t i = 0; i < AHEAD; ++i) {
+                const size_t p = first + paged_min(z0 + i * sets, nz - 1) * step;
+                f[i] = *(const float2 *)(ml + 2 * p);
+                v[i] = *(const float4v *)(po + p * D + 4 * d);
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < AHEAD; ++i)
+                if (z0 + i * sets < nz) add(f[i].x, f[i].y, v[i]);
+        }
+    }
+    if (sets > 1) {   // block-uniform
+        part[tid] = o;
+        if (d == 0) stat[team] = make_float2(M, l);
+        __syncthreads();
+        if (set) return;
+        for (uint32_t i = 1; i < sets; ++i) {
+            const float2 f = stat[team + i];
+            add(f.x, f.y, part[tid + i * LANES]);
+        }
+    }
+    if (!mine) return;
+    o *= l == 0.f ? 0.f : 1.f / l;
     *(uint2 *)(out + 4 * d) = make_uint2(pack2<BF>(o[0], o[1]), pack2<BF>(o[2], o[3]));
     if (lse && d == 0) *lse = l == 0.f ? -INFINITY : (M + __builtin_amdgcn_logf(l)) * LN2;
 }
 
-// Block = a row: of (sequence, KV head) for few_part's, of (row tile, KV head)
-// for chunk_part's, which come after.
 template <int D, bool BF>
-__global__ __launch_bounds__(256) void join_kernel(AttnArgs a, uint32_t few_rows_blocks) {
-    const uint32_t hkv = a.b.hkv;
-    if (blockIdx.x < few_rows_blocks) {
-        const uint32_t r = blockIdx.x % a.few_rows, unit = blockIdx.x / a.few_rows, kvh = unit % hkv, s = unit / hkv;
-        const PagedSeq sq = paged_seq(a.b, s);
-        const uint32_t n = paged_min(sq.n, a.b.max_q), R = n * a.G;
-        if (r >= R || R > FEW) return;
-        const uint32_t prefix = a.prefix ? a.prefix[s] : 0u;
-        const uint32_t lo = paged_span(sq.first, sq.len, prefix, a.window).lo & ~31u;
-        const uint32_t hi = paged_span(sq.first + (int32_t)n - 1, sq.len, prefix, a.window).hi;
-        const uint32_t steps = hi > lo ? (hi - lo + 31) / 32 : 0;
-        if (steps <= a.few_steps) return;
-        const size_t row = sq.row0 + r / a.G;
-        const uint32_t head = kvh * a.G + r % a.G;
-        join_parts<D, BF>(a.few_o, a.few_ml, (size_t)unit * a.few_splits * a.few_rows + r, a.few_rows,
-                          (steps + a.few_steps - 1) / a.few_steps, a.out + row * a.o_stride + head * D,
-                          a.lse ? a.lse + row * a.hq + head : nullptr);
-        return;
+__global__ __launch_bounds__(256) void join_kernel(AttnArgs a, JoinArgs j) {
+    constexpr uint32_t TEAMS = 256 / (D / 4);
+    const uint32_t hkv = a.b.hkv, team = threadIdx.x / (D / 4);
+    const uint32_t few_blocks = (uint32_t)(j.few_rows / (TEAMS / j.few_sets));
+    bool mine = false;
+    size_t first = 0, step = 0, row = 0;
+    uint32_t nz = 0, head = 0, sets;
+    const float *po, *ml;
+    if (blockIdx.x < few_blocks) {
+        sets = j.few_sets;
+        po = a.few_o;
+        ml = a.few_ml;
+        const uint32_t i = blockIdx.x * (TEAMS / sets) + team / sets;
+        const uint32_t r = i % a.few_rows, unit = i / a.few_rows, kvh = unit % hkv, s = unit / hkv;
+        if (s < a.b.num_seqs) {
+            const PagedSeq sq = paged_seq(a.b, s);
+            const uint32_t n = paged_min(sq.n, a.b.max_q), R = n * a.G;
+            const uint32_t prefix = a.prefix ? a.prefix[s] : 0u;
+            const uint32_t lo = paged_span(sq.first, sq.len, prefix, a.window).lo & ~31u;
+            const uint32_t hi = paged_span(sq.first + (int32_t)n - 1, sq.len, prefix, a.window).hi;
+            const uint32_t steps = hi > lo ? (hi - lo + 31) / 32 : 0;
+            mine = r < R && R <= FEW && steps > a.few_steps;
+            nz = (steps + a.few_steps - 1) / a.few_steps;
+            first = (size_t)unit * a.few_splits * a.few_rows + r;
+            step = a.few_rows;
+            row = sq.row0 + r / a.G;
+            head = kvh * a.G + r % a.G;
+        }
+    } else {
+        sets = j.chunk_sets;
+        po = a.chunk_o;
+        ml = a.chunk_ml;
+        const uint32_t per = TEAMS / sets, block = blockIdx.x - few_blocks;   // rows of a block: in one tile
+        const uint32_t unit = block / (TILE_ROWS / per), r = block % (TILE_ROWS / per) * per + team / sets;
+        const uint32_t kvh = unit % hkv;
+        uint32_t s, tile;
+        if (!find_tile(a, unit / hkv, &s, &tile)) return;   // block-uniform
+        const RowTile rt = row_tile(a, s, tile);
+        if (rt.nz == 1) return;
+        mine = rt.r0 + r < rt.R;
+        nz = rt.nz;
+        first = (size_t)unit * a.chunk_splits * TILE_ROWS + r;
+        step = TILE_ROWS;
+        row = rt.sq.row0 + (rt.r0 + r) / a.G;
+        head = kvh * a.G + (rt.r0 + r) % a.G;
     }
-    const uint32_t block = blockIdx.x - few_rows_blocks, r = block % TILE_ROWS, unit = block / TILE_ROWS;
-    const uint32_t kvh = unit % hkv, u = unit / hkv;
-    uint32_t s, tile;
-    if (!find_tile(a, u, &s, &tile)) return;
-    const RowTile rt = row_tile(a, s, tile);
-    if (rt.nz == 1 || rt.r0 + r >= rt.R) return;
-    const size_t row = rt.sq.row0 + (rt.r0 + r) / a.G;
-    const uint32_t head = kvh * a.G + (rt.r0 + r) % a.G;
-    join_parts<D, BF>(a.chunk_o, a.chunk_ml, (size_t)unit * a.chunk_splits * TILE_ROWS + r, TILE_ROWS, rt.nz,
-                      a.out + row * a.o_stride + head * D, a.lse ? a.lse + row * a.hq + head : nullptr);
+    join_parts<D, BF>(po, ml, first, step, nz, sets, mine, a.out + row * a.o_stride + head * D,
+                      a.lse ? a.lse + row * a.hq + head : nullptr);
 }
 
 // ------------------------------------------------------------------- launch
@@ -764,9 +814,14 @@ void start(hipStream_t stream, const Plan &p, AttnArgs a, float *ws) {
     if (!chunk_blocks) attn_kernel<D, BF, GEN, FEW_ONLY><<<a.few_blocks, 256, 0, stream>>>(a);
     else if (!a.few_blocks) attn_kernel<D, BF, GEN, CHUNK_ONLY><<<chunk_blocks, 256, 0, stream>>>(a);
     else attn_kernel<D, BF, GEN, BOTH><<<a.few_blocks + chunk_blocks, 256, 0, stream>>>(a);
-    const uint32_t few_join = p.few_parts ? a.b.num_seqs * hkv * p.few_rows : 0;
-    const uint32_t chunk_join = p.chunk_parts ? p.units * hkv * TILE_ROWS : 0;
-    if (few_join + chunk_join) join_kernel<D, BF><<<few_join + chunk_join, 256, 0, stream>>>(a, few_join);
+    if (!p.few_parts && !p.chunk_parts) return;
+    auto sets_of = [](uint32_t splits) { return splits > 32 ? 8u : splits > 8 ? 4u : splits > 4 ? 2u : 1u; };
+    constexpr uint32_t TEAMS = 256 / (D / 4);
+    JoinArgs j{0, sets_of(p.few_splits), sets_of(p.chunk_splits)};
+    const uint32_t per = TEAMS / j.few_sets;   // few_part's rows of a block
+    if (p.few_parts) j.few_rows = ((uint64_t)a.b.num_seqs * hkv * p.few_rows + per - 1) / per * per;
+    const uint32_t chunk_join = p.chunk_parts ? p.units * hkv * TILE_ROWS / (TEAMS / j.chunk_sets) : 0;
+    join_kernel<D, BF><<<(uint32_t)(j.few_rows / per) + chunk_join, 256, 0, stream>>>(a, j);
 }
 
 template <int D, bool BF>

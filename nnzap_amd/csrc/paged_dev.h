@@ -54,13 +54,16 @@ __device__ __forceinline__ float2 paged_cos_sin(int32_t p, const double *inv_fre
 }
 
 // A table entry through the scalar cache (the table does not change while the
-// kernel runs); num_pages where there is no page or the keys are not wanted.
-__device__ __forceinline__ uint32_t paged_entry(const PagedView &b, uint32_t s, uint32_t key, bool wanted) {
-    const uint32_t e = key >> b.shift;
-    if (!wanted || e >= b.width) return b.num_pages;
+// kernel runs), as it stands there: it names a page only if it is below
+// num_pages.  Positions behind the table read its last entry.
+__device__ __forceinline__ uint32_t paged_raw(const PagedView &b, uint32_t s, uint32_t key) {
     typedef const uint32_t __attribute__((address_space(4))) *table_t;
     const table_t t = (table_t)(uintptr_t)(b.table + (size_t)s * b.width);
-    return paged_min(t[e], b.num_pages);
+    return t[paged_min(key >> b.shift, b.width - 1)];
+}
+// num_pages where there is no page or the key is not wanted.
+__device__ __forceinline__ uint32_t paged_entry(const PagedView &b, uint32_t s, uint32_t key, bool wanted) {
+    return wanted && key >> b.shift < b.width ? paged_min(paged_raw(b, s, key), b.num_pages) : b.num_pages;
 }
 
 // Unit u of a batch whose sequence i has count(i) units: which sequence's, and
