@@ -410,12 +410,17 @@ __device__ __forceinline__ void chunk_part(const AttnArgs &a, uint32_t block, Ch
     const int32_t pos = rt.sq.first + (int32_t)tok;
     const float slope = GEN && a.slopes ? a.slopes[head] * LOG2E : 0.f;
 
-    // Piece i of this thread: 16 bytes of K row krow(i), of V's group the same;
-    // a wave's pieces lie in one group of 16 keys, hence in one page.
-    constexpr int RPW = 64 / PIECES;   // K rows of a wave's piece
-    const uint32_t krow = (uint32_t)lane / PIECES + (uint32_t)wave * RPW;
-    const uint32_t koff = ((krow & 15) * D + 8 * (((uint32_t)lane % PIECES) ^ (krow & (PIECES - 1)))) * 2u;
-    const uint32_t vp = ((uint32_t)tid) % (2 * D), voff = ((vp / 2) << a.b.shift) * 2u + (vp & 1) * 16u;
+    // Wave w stages group w of a tile's four groups of 16 keys, K and V alike:
+    // one page.  Piece i of a lane: 16 bytes of K row 64 i / PIECES + lane / PIECES,
+    // of V^T row 32 i + lane / 2.
+    constexpr uint32_t RPW = 64 / PIECES;   // K rows of the wave's piece
+    uint32_t koff[LOADS], voff[LOADS];
+#pragma unroll
+    for (uint32_t i = 0; i < LOADS; ++i) {
+        const uint32_t row = i * RPW + (uint32_t)lane / PIECES;
+        koff[i] = (row * D + 8 * (((uint32_t)lane % PIECES) ^ (row & (PIECES - 1)))) * 2u;
+        voff[i] = ((32 * i + (uint32_t)lane / 2) << a.b.shift) * 2u + ((uint32_t)lane & 1) * 16u;
+    }
     // elements of a page; this head's part of page 0
     const uint32_t pmask = (1u << a.b.shift) - 1, page_len = (hkv * D) << a.b.shift;
     const uint16_t *const kh = a.k + (((size_t)kvh * D) << a.b.shift), *const vh = a.v + (((size_t)kvh * D) << a.b.shift);
@@ -429,27 +434,20 @@ __device__ __forceinline__ void chunk_part(const AttnArgs &a, uint32_t block, Ch
         return p;
     };
     auto has_page = [&](const Pages &p, uint32_t t, int i) { return t * KT + 16 * i < rt.hi && p.p[i] < a.b.num_pages; };
-    auto stage = [&](uint32_t t, const Pages &p) __attribute__((always_inline)) {
-        const uint32_t k0 = t * KT, buf = t & 1;
-        const uint32_t lk = __builtin_amdgcn_readfirstlane(
-            (uint32_t)(size_t)(__attribute__((address_space(3))) uint16_t *)(sh.k[buf] + 8 * 64 * wave));
-        const uint32_t lv = __builtin_amdgcn_readfirstlane(
-            (uint32_t)(size_t)(__attribute__((address_space(3))) uint16_t *)(sh.v[buf] + 8 * 64 * wave));
+    const uint32_t lds_k = __builtin_amdgcn_readfirstlane(
+        (uint32_t)(size_t)(__attribute__((address_space(3))) uint16_t *)(sh.k[0] + 16 * D * wave));
+    const uint32_t lds_v = __builtin_amdgcn_readfirstlane(
+        (uint32_t)(size_t)(__attribute__((address_space(3))) uint16_t *)(sh.v[0] + 16 * D * wave));
+    auto stage = [&](uint32_t t, uint32_t entry) __attribute__((always_inline)) {
+        const uint32_t key = t * KT + 16 * (uint32_t)wave, buf = (t & 1) * (TILE * 2);
+        // any page where there is none: the keys are masked
+        const uint32_t page = key < rt.hi && entry < a.b.num_pages ? entry : 0u, slot = key & pmask;
+        const uint64_t at = (uint64_t)page * page_len;
+        const uint16_t *const kp = kh + at + slot * D, *const vp = vh + at + slot;
 #pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-            uint32_t page, in;   // any page where there is none: the keys are masked
-            if constexpr (D == 128) {
-                page = has_page(p, t, i) ? p.p[i] : 0u;
-                in = 16 * i;
-            } else {   // a piece index spans two groups
-                const uint32_t lower = has_page(p, t, 2 * i) ? p.p[2 * i] : 0u, upper = has_page(p, t, 2 * i + 1) ? p.p[2 * i + 1] : 0u;
-                page = wave < 2 ? lower : upper;
-                in = 32 * i + (wave < 2 ? 0 : 16);
-            }
-            const uint64_t at = (uint64_t)page * page_len;
-            const uint32_t slot = (k0 + in) & pmask;
-            load_to_lds(kh + at + slot * D, koff, lk + 16u * (uint32_t)(i * 256));
-            load_to_lds(vh + at + slot, voff, lv + 16u * (uint32_t)(i * 256));
+        for (uint32_t i = 0; i < LOADS; ++i) {
+            load_to_lds(kp, koff[i], lds_k + buf + 1024 * i);
+            load_to_lds(vp, voff[i], lds_v + buf + 1024 * i);
         }
     };
     auto bad_of = [&](const Pages &p, uint32_t t) __attribute__((always_inline)) {
@@ -459,11 +457,14 @@ __device__ __forceinline__ void chunk_part(const AttnArgs &a, uint32_t block, Ch
         return bad;
     };
 
+    // table entries: this wave's of the next tile, all of this one and the next
     Pages cur{}, next{};
+    uint32_t ahead_entry = 0;
     if (t0 < t1) {
         cur = pages_of(t0);
-        stage(t0, cur);
+        stage(t0, paged_raw(a.b, s, t0 * KT + 16 * (uint32_t)wave));
         next = pages_of(t0 + 1);
+        ahead_entry = paged_raw(a.b, s, (t0 + 1) * KT + 16 * (uint32_t)wave);
     }
     v4u qf[NKS];
     {
@@ -491,9 +492,10 @@ __device__ __forceinline__ void chunk_part(const AttnArgs &a, uint32_t block, Ch
         asm volatile("" ::: "memory");
         const uint32_t bad = bad_of(cur, t);
         if (t + 1 < t1) {   // block-uniform
-            stage(t + 1, next);
+            stage(t + 1, ahead_entry);
             cur = next;
             next = pages_of(t + 2);
+            ahead_entry = paged_raw(a.b, s, (t + 2) * KT + 16 * (uint32_t)wave);
         }
         const uint16_t *const Kt = sh.k[t & 1], *const Vt = sh.v[t & 1];
         const uint32_t k0 = t * KT;
