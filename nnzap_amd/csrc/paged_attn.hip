@@ -15,8 +15,8 @@
 //               registers, each byte once; keys are split over waves and blocks;
 //   chunk_part  more rows (chunks of prompts): bound by the matrix cores and the
 //               softmax's vector work beside them; 128 rows a block, K and V
-//               tiles of 64 keys in LDS, two buffers; keys are split over blocks
-//               where there are few rows.
+//               tiles of 64 keys in LDS; keys are split over two groups of waves,
+//               and over blocks where there are few rows.
 // join_kernel joins what blocks computed of one row.
 //
 // The softmax is the online one in base 2: sums are kept relative to a
@@ -123,7 +123,7 @@ __device__ __forceinline__ float general_score(const AttnArgs &a, float s, float
 // A step is 32 keys of a wave: K as two A operands of 16 keys (row m of operand
 // i is key 8 (m >> 2) + 4 i + (m & 3), so lane group g's accumulators hold keys
 // 8 g .. 8 g + 7), V^T as D/16 A operands.  The next step's loads are issued
-// before the current one is computed.  Block = 4 waves that take the steps of
+// before the current one is computed.  Block = W waves that take the steps of
 // a chunk in turn.
 template <int D, bool BF>
 struct FewStep {
@@ -131,14 +131,14 @@ struct FewStep {
     uint32_t bad;   // groups of 16 keys without a page
 };
 
-template <int D>
+template <int D, int W>
 struct FewShared {
-    float4v o[4][D / 16][64];
-    float m[4][16], l[4][16];
+    float4v o[W][D / 16][64];
+    float m[W][16], l[W][16];
 };
 
-template <int D, bool BF, bool GEN>
-__device__ __forceinline__ void few_part(const AttnArgs &a, uint32_t block, FewShared<D> &sh) {
+template <int D, bool BF, bool GEN, int W>
+__device__ __forceinline__ void few_part(const AttnArgs &a, uint32_t block, FewShared<D, W> &sh) {
     constexpr int NKS = D / 32, NDT = D / 16;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, c = lane & 15;
@@ -254,18 +254,18 @@ __device__ __forceinline__ void few_part(const AttnArgs &a, uint32_t block, FewS
         FewStep<D, BF> f0, f1;
         load(f0, st);
         for (;;) {
-            if (st + 4 < st1) load(f1, st + 4);
+            if (st + W < st1) load(f1, st + W);
             compute(f0, st);
-            st += 4;
+            st += W;
             if (st >= st1) break;
-            if (st + 4 < st1) load(f0, st + 4);
+            if (st + W < st1) load(f0, st + W);
             compute(f1, st);
-            st += 4;
+            st += W;
             if (st >= st1) break;
         }
     }
     if (__builtin_expect(__builtin_amdgcn_ballot_w64(odd != 0) != 0, 0)) {   // wave-uniform
-        for (st = z * a.few_steps + (uint32_t)w; st < st1; st += 4) {
+        for (st = z * a.few_steps + (uint32_t)w; st < st1; st += W) {
             const uint32_t k0 = lo + 32 * st;
             const bool hole = paged_entry(a.b, s, k0, true) == a.b.num_pages ||
                               paged_entry(a.b, s, k0 + 16, k0 + 16 < hi) == a.b.num_pages;
@@ -286,7 +286,7 @@ __device__ __forceinline__ void few_part(const AttnArgs &a, uint32_t block, FewS
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
 
-    // the four waves' parts, relative to the largest reference
+    // the waves' parts, relative to the largest reference
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt) sh.o[w][dt][lane] = o[dt];
     if (g == 0) {
@@ -294,12 +294,12 @@ __device__ __forceinline__ void few_part(const AttnArgs &a, uint32_t block, FewS
         sh.l[w][c] = l;
     }
     __syncthreads();
-    float M = sh.m[0][c], wt[4];
+    float M = sh.m[0][c], wt[W];
 #pragma unroll
-    for (int i = 1; i < 4; ++i) M = fmaxf(M, sh.m[i][c]);
+    for (int i = 1; i < W; ++i) M = fmaxf(M, sh.m[i][c]);
     l = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < W; ++i) {
         wt[i] = sh.m[i][c] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sh.m[i][c] - M);
         l += wt[i] * sh.l[i][c];   // NaN stays NaN, times 0 too
     }
@@ -309,10 +309,10 @@ __device__ __forceinline__ void few_part(const AttnArgs &a, uint32_t block, FewS
         uint16_t *op = a.out + (sq.row0 + tok) * a.o_stride + head * D + 4 * g;
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt) {
-            if (dt % 4 != w) continue;
+            if (dt % W != w) continue;
             float4v t = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) t += sh.o[i][dt][lane] * wt[i];
+            for (int i = 0; i < W; ++i) t += sh.o[i][dt][lane] * wt[i];
             if (mine)
                 *(uint2 *)(op + 16 * dt) = make_uint2(pack2<BF>(t[0] * inv, t[1] * inv), pack2<BF>(t[2] * inv, t[3] * inv));
         }
@@ -323,10 +323,10 @@ __device__ __forceinline__ void few_part(const AttnArgs &a, uint32_t block, FewS
     const size_t part = (((size_t)s * hkv + kvh) * a.few_splits + z) * a.few_rows + (uint32_t)c;
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt) {
-        if (dt % 4 != w) continue;
+        if (dt % W != w) continue;
         float4v t = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) t += sh.o[i][dt][lane] * wt[i];
+        for (int i = 0; i < W; ++i) t += sh.o[i][dt][lane] * wt[i];
         if (mine) *(float4v *)(a.few_o + part * D + 16 * dt + 4 * g) = t;
     }
     if (mine && g == 0 && w == 0) {
@@ -377,9 +377,20 @@ __device__ __forceinline__ RowTile row_tile(const AttnArgs &a, uint32_t s, uint3
 // LDS with their 16-byte pieces rotated (piece p of row r at slot p ^ r), V as
 // its pages have it, [16-key group][dim][16 keys], where a wave's operand is
 // one contiguous run.
+//
+// The block's eight waves are two groups of four that hold the same rows and
+// take the key tiles in turn, half a tile apart: a SIMD has a wave of each, and
+// while one multiplies K and Q the other runs its softmax and the product with
+// V, so that matrix and vector instructions of the two overlap.  A barrier ends
+// every half.  At the end the second group's sums join the first's.
 template <int D>
 struct ChunkShared {
-    uint16_t k[2][KT * D], v[2][KT * D];
+    union {
+        struct {
+            uint16_t k[2][2][KT * D], v[2][2][KT * D];   // [group][buffer]
+        };
+        float join[4][D / 2 + 2][64];   // [wave][register][lane]
+    };
 };
 
 template <int D, bool BF, bool GEN>
@@ -387,7 +398,8 @@ __device__ __forceinline__ void chunk_part(const AttnArgs &a, uint32_t block, Ch
     constexpr int NKS = D / 16, NDT = D / 32, PIECES = D / 8;   // pieces of 16 bytes in a K row
     constexpr int TILE = KT * D, LOADS = TILE / 8 / 256;
     const int tid = threadIdx.x, lane = tid & 63, hh = lane >> 5, c = lane & 31;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t group = __builtin_amdgcn_readfirstlane(tid >> 8);
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6 & 3);
     // KV head fastest: with 8 of them each XCD keeps one head's K and V in its L2;
     // the last tiles, which see the most keys, first
     const uint32_t hkv = a.b.hkv, kvh = block % hkv, z = block / hkv % a.chunk_splits;
@@ -435,11 +447,11 @@ __device__ __forceinline__ void chunk_part(const AttnArgs &a, uint32_t block, Ch
     };
     auto has_page = [&](const Pages &p, uint32_t t, int i) { return t * KT + 16 * i < rt.hi && p.p[i] < a.b.num_pages; };
     const uint32_t lds_k = __builtin_amdgcn_readfirstlane(
-        (uint32_t)(size_t)(__attribute__((address_space(3))) uint16_t *)(sh.k[0] + 16 * D * wave));
+        (uint32_t)(size_t)(__attribute__((address_space(3))) uint16_t *)(sh.k[group][0] + 16 * D * wave));
     const uint32_t lds_v = __builtin_amdgcn_readfirstlane(
-        (uint32_t)(size_t)(__attribute__((address_space(3))) uint16_t *)(sh.v[0] + 16 * D * wave));
-    auto stage = [&](uint32_t t, uint32_t entry) __attribute__((always_inline)) {
-        const uint32_t key = t * KT + 16 * (uint32_t)wave, buf = (t & 1) * (TILE * 2);
+        (uint32_t)(size_t)(__attribute__((address_space(3))) uint16_t *)(sh.v[group][0] + 16 * D * wave));
+    auto stage = [&](uint32_t t, uint32_t entry, uint32_t half) __attribute__((always_inline)) {
+        const uint32_t key = t * KT + 16 * (uint32_t)wave, buf = half * (TILE * 2);
         // any page where there is none: the keys are masked
         const uint32_t page = key < rt.hi && entry < a.b.num_pages ? entry : 0u, slot = key & pmask;
         const uint64_t at = (uint64_t)page * page_len;
@@ -457,14 +469,15 @@ __device__ __forceinline__ void chunk_part(const AttnArgs &a, uint32_t block, Ch
         return bad;
     };
 
-    // table entries: this wave's of the next tile, all of this one and the next
+    // table entries: this wave's of the group's next tile, all of this one and the next
+    const uint32_t ta = t0 + group;
     Pages cur{}, next{};
     uint32_t ahead_entry = 0;
-    if (t0 < t1) {
-        cur = pages_of(t0);
-        stage(t0, paged_raw(a.b, s, t0 * KT + 16 * (uint32_t)wave));
-        next = pages_of(t0 + 1);
-        ahead_entry = paged_raw(a.b, s, (t0 + 1) * KT + 16 * (uint32_t)wave);
+    if (ta < t1) {
+        cur = pages_of(ta);
+        stage(ta, paged_raw(a.b, s, ta * KT + 16 * (uint32_t)wave), 0);
+        next = pages_of(ta + 2);
+        ahead_entry = paged_raw(a.b, s, (ta + 2) * KT + 16 * (uint32_t)wave);
     }
     v4u qf[NKS];
     {
@@ -483,23 +496,31 @@ __device__ __forceinline__ void chunk_part(const AttnArgs &a, uint32_t block, Ch
     auto in_part = [&](uint32_t k0, uint32_t gone) { return k0 < last.lo || k0 + KT > first.hi || gone; };   // wave-uniform
     const int krm = (c & 19) | ((c & 4) << 1) | ((c & 8) >> 1);   // key of A row c
 
-    for (uint32_t t = t0; t < t1; ++t) {
-        // this tile's loads have arrived, everybody's, and nobody reads the
-        // other buffer any more
-        __builtin_amdgcn_s_waitcnt(7 << 4);   // vmcnt 0, lgkmcnt 0
+    auto barrier = [&]() __attribute__((always_inline)) {
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
+    };
+    const uint32_t turns = (t1 - t0 + 1) / 2;   // of both groups; the second's last tile may not be there
+    if (group) barrier();
+    for (uint32_t i = 0; i < turns; ++i) {
+        const uint32_t t = ta + 2 * i, k0 = t * KT;
+        // the group's loads of this tile have arrived, and its waves are done
+        // with the other buffer
+        __builtin_amdgcn_s_waitcnt(7 << 4);   // vmcnt 0, lgkmcnt 0
+        barrier();
         const uint32_t bad = bad_of(cur, t);
-        if (t + 1 < t1) {   // block-uniform
-            stage(t + 1, ahead_entry);
+        if (t + 2 < t1) {   // group-uniform
+            stage(t + 2, ahead_entry, (i + 1) & 1);
             cur = next;
-            next = pages_of(t + 2);
-            ahead_entry = paged_raw(a.b, s, (t + 2) * KT + 16 * (uint32_t)wave);
+            next = pages_of(t + 4);
+            ahead_entry = paged_raw(a.b, s, (t + 4) * KT + 16 * (uint32_t)wave);
         }
-        const uint16_t *const Kt = sh.k[t & 1], *const Vt = sh.v[t & 1];
-        const uint32_t k0 = t * KT;
-        if (!any || k0 >= last.hi || k0 + KT <= first.lo) continue;   // wave-uniform
+        if (t >= t1 || !any || k0 >= last.hi || k0 + KT <= first.lo) {   // wave-uniform
+            barrier();
+            continue;
+        }
+        const uint16_t *const Kt = sh.k[group][i & 1], *const Vt = sh.v[group][i & 1];
         // scores of both halves of the tile; the operands of a half are all read
         // before its products, the second half's during the first one's
         float16v sc[2];
@@ -527,6 +548,7 @@ __device__ __forceinline__ void chunk_part(const AttnArgs &a, uint32_t block, Ch
         };
         read_v(0);
         __builtin_amdgcn_sched_barrier(0);
+        barrier();
         const uint32_t key = k0 + 8 * hh;   // register e of half kt: key + 32 kt + 16 (e >> 3) + (e & 7)
         if constexpr (GEN) {
 #pragma unroll
@@ -579,8 +601,9 @@ __device__ __forceinline__ void chunk_part(const AttnArgs &a, uint32_t block, Ch
             if (st < 3) read_v(st + 1);
         }
     }
+    if (!group) barrier();
     if (__builtin_expect(__builtin_amdgcn_ballot_w64(odd != 0) != 0, 0)) {   // wave-uniform
-        for (uint32_t t = t0; t < t1; ++t) {
+        for (uint32_t t = ta; t < t1; t += 2) {
             const uint32_t k0 = t * KT;
             if (!in_part(k0, bad_of(pages_of(t), t))) continue;   // whole tiles had V as it is
             for (uint32_t key = k0; key < k0 + KT; ++key) {
@@ -598,8 +621,30 @@ __device__ __forceinline__ void chunk_part(const AttnArgs &a, uint32_t block, Ch
     }
     const float2 lp = swap32(l, l);
     l = lp.x + lp.y;
-    if (!any || w0 + (uint32_t)c >= rt.R) return;
-    const float M = -nm;
+    float M = m == -INFINITY ? -INFINITY : -nm;
+    __syncthreads();
+    float (&join)[D / 2 + 2][64] = sh.join[wave];
+    if (group) {
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) join[16 * dt + e][lane] = o[dt][e];
+        join[D / 2][lane] = M;
+        join[D / 2 + 1][lane] = l;
+    }
+    __syncthreads();
+    if (group || !any || w0 + (uint32_t)c >= rt.R) return;
+    {
+        const float M2 = join[D / 2][lane], to = fmaxf(M, M2);
+        const float f = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - to);
+        const float f2 = M2 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M2 - to);
+        l = l * f + join[D / 2 + 1][lane] * f2;
+        M = to;
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[dt][e] = o[dt][e] * f + join[16 * dt + e][lane] * f2;
+    }
     if (rt.nz > 1) {
         const size_t part = (((size_t)u * hkv + kvh) * a.chunk_splits + z) * TILE_ROWS + (w0 - rt.r0) + (uint32_t)c;
 #pragma unroll
@@ -609,7 +654,7 @@ __device__ __forceinline__ void chunk_part(const AttnArgs &a, uint32_t block, Ch
                 *(float4v *)(a.chunk_o + part * D + 32 * dt + 8 * j + 4 * hh) =
                     (float4v){o[dt][4 * j], o[dt][4 * j + 1], o[dt][4 * j + 2], o[dt][4 * j + 3]};
         if (hh == 0) {
-            a.chunk_ml[2 * part] = m == -INFINITY ? -INFINITY : M;
+            a.chunk_ml[2 * part] = M;
             a.chunk_ml[2 * part + 1] = l;
         }
         return;
@@ -629,17 +674,19 @@ __device__ __forceinline__ void chunk_part(const AttnArgs &a, uint32_t block, Ch
 
 // One launch for a batch: few_part's blocks first (they wait for memory while
 // the chunks' compute).
-enum { FEW_ONLY, CHUNK_ONLY, BOTH };
+enum { FEW_4, FEW_8, CHUNK, BOTH };   // few_part by 4 or 8 waves, chunk_part, both
+constexpr int threads_of(int kind) { return kind == FEW_4 ? 256 : 512; }
 template <int D, bool BF, bool GEN, int KIND>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void attn_kernel(AttnArgs a) {
+__global__ __launch_bounds__(threads_of(KIND)) __attribute__((amdgpu_waves_per_eu(2))) void attn_kernel(AttnArgs a) {
+    constexpr int W = threads_of(KIND) / 64;
     __shared__ __align__(16) union {
         char none;
-        typename std::conditional<KIND != CHUNK_ONLY, FewShared<D>, char>::type few;
-        typename std::conditional<KIND != FEW_ONLY, ChunkShared<D>, char>::type chunk;
+        typename std::conditional<KIND != CHUNK, FewShared<D, W>, char>::type few;
+        typename std::conditional<KIND == CHUNK || KIND == BOTH, ChunkShared<D>, char>::type chunk;
     } sh;
-    if constexpr (KIND == FEW_ONLY) few_part<D, BF, GEN>(a, blockIdx.x, sh.few);
-    else if constexpr (KIND == CHUNK_ONLY) chunk_part<D, BF, GEN>(a, blockIdx.x, sh.chunk);
-    else if (blockIdx.x < a.few_blocks) few_part<D, BF, GEN>(a, blockIdx.x, sh.few);
+    if constexpr (KIND == CHUNK) chunk_part<D, BF, GEN>(a, blockIdx.x, sh.chunk);
+    else if constexpr (KIND != BOTH) few_part<D, BF, GEN, W>(a, blockIdx.x, sh.few);
+    else if (blockIdx.x < a.few_blocks) few_part<D, BF, GEN, W>(a, blockIdx.x, sh.few);
     else chunk_part<D, BF, GEN>(a, blockIdx.x - a.few_blocks, sh.chunk);
 }
 
@@ -771,7 +818,7 @@ Plan plan_of(const nnz_paged_kv &kv, const nnz_paged_batch &b, uint32_t hq) {
     // length turns out to be; a batch of several may hold both kinds.
     if (G <= FEW && (!chunks || b.num_seqs > 1)) {
         const uint32_t steps = (b.max_kv_len + 31) / 32, blocks = b.num_seqs * hkv;   // below 2^26
-        const uint32_t want = std::max(1u, (chunks ? 512u : 1024u) / blocks), most_splits = std::max(1u, steps / 16);
+        const uint32_t want = std::max(1u, (chunks ? 256u : 1024u) / blocks), most_splits = std::max(1u, steps / 16);
         const uint32_t splits = std::min({want, most_splits, MOST_SPLITS});
         p.few_rows = (uint32_t)std::min<uint64_t>(most, FEW);
         p.few_steps = (steps + splits - 1) / splits;
@@ -783,7 +830,7 @@ Plan plan_of(const nnz_paged_kv &kv, const nnz_paged_batch &b, uint32_t hq) {
         const uint64_t by_seqs = (uint64_t)b.num_seqs * ((most + TILE_ROWS - 1) / TILE_ROWS);
         p.units = (uint32_t)std::min(by_rows, by_seqs);
         const uint32_t tiles = (b.max_kv_len + KT - 1) / KT;
-        const uint32_t want = (uint32_t)std::max<uint64_t>(1, 512 / ((uint64_t)p.units * hkv)), most_splits = std::max(1u, tiles / 4);
+        const uint32_t want = (uint32_t)std::max<uint64_t>(1, 256 / ((uint64_t)p.units * hkv)), most_splits = std::max(1u, tiles / 4);
         const uint32_t splits = std::min({want, most_splits, MOST_SPLITS});
         p.chunk_tiles = (tiles + splits - 1) / splits;
         p.chunk_splits = (tiles + p.chunk_tiles - 1) / p.chunk_tiles;
@@ -813,9 +860,10 @@ void start(hipStream_t stream, const Plan &p, AttnArgs a, float *ws) {
     a.chunk_o = a.few_ml + p.few_parts * 2;
     a.chunk_ml = a.chunk_o + p.chunk_parts * D;
     const uint32_t chunk_blocks = p.units * hkv * p.chunk_splits;
-    if (!chunk_blocks) attn_kernel<D, BF, GEN, FEW_ONLY><<<a.few_blocks, 256, 0, stream>>>(a);
-    else if (!a.few_blocks) attn_kernel<D, BF, GEN, CHUNK_ONLY><<<chunk_blocks, 256, 0, stream>>>(a);
-    else attn_kernel<D, BF, GEN, BOTH><<<a.few_blocks + chunk_blocks, 256, 0, stream>>>(a);
+    if (!chunk_blocks && a.few_blocks > 256) attn_kernel<D, BF, GEN, FEW_4><<<a.few_blocks, 256, 0, stream>>>(a);
+    else if (!chunk_blocks) attn_kernel<D, BF, GEN, FEW_8><<<a.few_blocks, 512, 0, stream>>>(a);
+    else if (!a.few_blocks) attn_kernel<D, BF, GEN, CHUNK><<<chunk_blocks, 512, 0, stream>>>(a);
+    else attn_kernel<D, BF, GEN, BOTH><<<a.few_blocks + chunk_blocks, 512, 0, stream>>>(a);
     if (!p.few_parts && !p.chunk_parts) return;
     auto sets_of = [](uint32_t splits) { return splits > 32 ? 8u : splits > 8 ? 4u : splits > 4 ? 2u : 1u; };
     constexpr uint32_t TEAMS = 256 / (D / 4);
