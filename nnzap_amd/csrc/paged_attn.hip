@@ -391,6 +391,7 @@ struct ChunkShared {
         };
         float join[4][D / 2 + 2][64];   // [wave][register][lane]
     };
+    uint32_t odd[2][4];   // [group][wave]
 };
 
 template <int D, bool BF, bool GEN>
@@ -493,7 +494,10 @@ __device__ __forceinline__ void chunk_part(const AttnArgs &a, uint32_t block, Ch
     const float cs = GEN ? 1.f : a.scale, ahead = 8.f / cs;
     float m = -INFINITY, nm = 0.f, l = 0.f;
     uint32_t odd = 0;
-    auto in_part = [&](uint32_t k0, uint32_t gone) { return k0 < last.lo || k0 + KT > first.hi || gone; };   // wave-uniform
+    // tiles that some rows of the wave, of the block, see only in part
+    auto in_part = [&](uint32_t k0, uint32_t gone) { return k0 < last.lo || k0 + KT > first.hi || gone; };
+    const uint32_t lo_most = span_of(paged_min(rt.r0 + TILE_ROWS, rt.R) - 1).lo, hi_least = span_of(rt.r0).hi;
+    auto block_part = [&](uint32_t k0, uint32_t gone) { return k0 < lo_most || k0 + KT > hi_least || gone; };
     const int krm = (c & 19) | ((c & 4) << 1) | ((c & 8) >> 1);   // key of A row c
 
     auto barrier = [&]() __attribute__((always_inline)) {
@@ -508,8 +512,20 @@ __device__ __forceinline__ void chunk_part(const AttnArgs &a, uint32_t block, Ch
         // the group's loads of this tile have arrived, and its waves are done
         // with the other buffer
         __builtin_amdgcn_s_waitcnt(7 << 4);   // vmcnt 0, lgkmcnt 0
-        barrier();
         const uint32_t bad = bad_of(cur, t);
+        if (t < t1 && block_part(k0, bad)) {   // the 16 keys that this wave has staged
+            uint16_t *const mine = sh.v[group][i & 1] + 16 * D * wave + 8 * lane;
+#pragma unroll
+            for (int j = 0; j < LOADS; ++j) {
+                v4u *const at = (v4u *)(mine + 512 * j);
+                uint32_t met = 0;
+                const v4u v = finite_part<BF>(*at, met);
+                if (met) *at = v;
+                odd |= met;
+            }
+            __builtin_amdgcn_s_waitcnt(7 << 4);
+        }
+        barrier();
         if (t + 2 < t1) {   // group-uniform
             stage(t + 2, ahead_entry, (i + 1) & 1);
             cur = next;
@@ -581,31 +597,48 @@ __device__ __forceinline__ void chunk_part(const AttnArgs &a, uint32_t block, Ch
 #pragma unroll
                 for (int e = 0; e < 16; ++e) o[dt][e] *= alpha;
         }
+        // Weights of two keys, and a word of the B operand of the 16 keys they are in
+        auto weigh = [&](int i) __attribute__((always_inline)) {
+            const float x = __builtin_amdgcn_exp2f(fmaf(sc[i >> 3][2 * (i & 7)], cs, nm));
+            const float y = __builtin_amdgcn_exp2f(fmaf(sc[i >> 3][2 * (i & 7) + 1], cs, nm));
+            l += x;
+            l += y;
+            return pack2<BF>(x, y);
+        };
+        // a wave issues in order: between the products of 16 keys come the weights
+        // of the next 16, or the vector unit would wait for the matrix cores, which
+        // the other group shares
+        v4u p, ahead_p = {};
 #pragma unroll
-        for (int st = 0; st < 4; ++st) {   // 16 keys each
-            v4u p;
+        for (int i = 0; i < 4; ++i) p[i] = weigh(i);
 #pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-                const float x = __builtin_amdgcn_exp2f(fmaf(sc[st >> 1][8 * (st & 1) + e], cs, nm));
-                const float y = __builtin_amdgcn_exp2f(fmaf(sc[st >> 1][8 * (st & 1) + e + 1], cs, nm));
-                l += x;
-                l += y;
-                p[e / 2] = pack2<BF>(x, y);
-            }
-            if (masked) {
+        for (int st = 0; st < 4; ++st) {
+            v4u v[NDT];
 #pragma unroll
-                for (int dt = 0; dt < NDT; ++dt) vf[dt] = finite_part<BF>(vf[dt], odd);
-            }
-#pragma unroll
-            for (int dt = 0; dt < NDT; ++dt) o[dt] = mfma32<BF>(vf[dt], p, o[dt]);
+            for (int dt = 0; dt < NDT; ++dt) v[dt] = vf[dt];
             if (st < 3) read_v(st + 1);
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt) {
+                o[dt] = mfma32<BF>(v[dt], p, o[dt]);
+                if (st < 3)
+#pragma unroll
+                    for (int i = dt * 4 / NDT; i < (dt + 1) * 4 / NDT; ++i) ahead_p[i] = weigh(4 * (st + 1) + i);
+                __builtin_amdgcn_sched_barrier(0);   // keep this order
+            }
+            p = ahead_p;
         }
     }
     if (!group) barrier();
-    if (__builtin_expect(__builtin_amdgcn_ballot_w64(odd != 0) != 0, 0)) {   // wave-uniform
+    const float2 lp = swap32(l, l);
+    l = lp.x + lp.y;
+    float M = m == -INFINITY ? -INFINITY : -nm;
+    if (lane == 0) sh.odd[group][wave] = 0;
+    if (odd) sh.odd[group][wave] = 1;   // after the store above, both by this wave
+    __syncthreads();
+    if (__builtin_expect(sh.odd[group][0] | sh.odd[group][1] | sh.odd[group][2] | sh.odd[group][3], 0)) {   // group-uniform
         for (uint32_t t = ta; t < t1; t += 2) {
             const uint32_t k0 = t * KT;
-            if (!in_part(k0, bad_of(pages_of(t), t))) continue;   // whole tiles had V as it is
+            if (!block_part(k0, bad_of(pages_of(t), t))) continue;   // whole tiles had V as it is
             for (uint32_t key = k0; key < k0 + KT; ++key) {
                 const uint32_t page = paged_entry(a.b, s, key, key < rt.hi);
                 if (page == a.b.num_pages) continue;
@@ -619,10 +652,6 @@ __device__ __forceinline__ void chunk_part(const AttnArgs &a, uint32_t block, Ch
             }
         }
     }
-    const float2 lp = swap32(l, l);
-    l = lp.x + lp.y;
-    float M = m == -INFINITY ? -INFINITY : -nm;
-    __syncthreads();
     float (&join)[D / 2 + 2][64] = sh.join[wave];
     if (group) {
 #pragma unroll
