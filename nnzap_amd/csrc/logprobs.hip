@@ -13,7 +13,7 @@
 //   * candidates for the best top_n.  A group of 16 values per lane is looked at
 //     again only if one of them reaches the wave's bound; the bound rises to a
 //     value that top_n of the lanes' maxima reach (top_n values of the row are
-//     no smaller: 16 ballots find its upper half), and what reaches it waits in
+//     no smaller: 12 ballots find sign, exponent and three bits), and what reaches it waits in
 //     LDS with its id.  Should more than 128 wait, they are sorted, 64 at a
 //     time, into a list of keys (value and complemented id: larger is earlier),
 //     whose last bounds what follows.  Ids rise along a wave's part, so that a
@@ -131,12 +131,13 @@ struct Sums {
     }
 };
 
-// A value that at least n lanes' x reach, a little below the n-th largest.
+// A value that at least n lanes' x reach, at most an eighth below the n-th
+// largest of them.
 __device__ __forceinline__ float reached_by(float x, uint32_t n) {
     const uint32_t u = __float_as_uint(x + 0.f), k = u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
     uint32_t f = 0;
 #pragma unroll
-    for (int b = 31; b >= 16; --b) {
+    for (int b = 31; b >= 20; --b) {
         const uint32_t up = f | 1u << b;
         f = __builtin_popcountll(__builtin_amdgcn_ballot_w64(k >= up)) >= (int)n ? up : f;
     }
@@ -383,17 +384,20 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(LpArgs a) {
     __shared__ uint64_t reach[WAVES];
     __shared__ uint32_t count;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), row = blockIdx.x;
-    const uint32_t tok = a.tokens[row];
-    const bool named = tok < a.vocab;
-    const float xt = named ? load_as_f32<DT>(a.x, (size_t)row * a.stride + tok) : 0.f;
     const float4 *const part = a.part + (size_t)row * a.pieces;
     const uint64_t *const keys = a.part_keys + (size_t)row * a.pieces * a.top;
+    const uint32_t nk = a.pieces * a.top, tok = a.tokens[row];
+    // every load at once: the first part of a lane, the pieces' last keys (at most
+    // 96, a thread each), the first four keys of a thread
+    const float4 first = lane < a.pieces ? part[lane] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+    const uint64_t last = a.top && tid < a.pieces ? keys[(size_t)tid * a.top + a.top - 1] : 0;
+    uint64_t mine[4];
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) mine[i] = tid + 256 * i < nk ? keys[tid + 256 * i] : 0;
+    const bool named = tok < a.vocab;
+    const float xt = named ? load_as_f32<DT>(a.x, (size_t)row * a.stride + tok) : 0.f;
     if (a.top) {
-        uint64_t k = 0;
-        for (uint32_t p = tid; p < a.pieces; p += 256) {
-            const uint64_t last = keys[(size_t)p * a.top + a.top - 1];
-            k = last > k ? last : k;
-        }
+        uint64_t k = last;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
             const uint64_t v = __shfl_xor((unsigned long long)k, o);
@@ -404,17 +408,19 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(LpArgs a) {
         __syncthreads();
 #pragma unroll
         for (uint32_t i = 0; i < WAVES; ++i) k = reach[i] > k ? reach[i] : k;
-        for (uint32_t i = tid; i < a.pieces * a.top; i += 256) {
-            const uint64_t v = keys[i];
+        auto put = [&](uint64_t v) {
             if (v && v >= k) kept[atomicAdd(&count, 1u)] = v;   // any order: they are sorted next
-        }
+        };
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) put(mine[i]);
+        for (uint32_t i = tid + 1024; i < nk; i += 256) put(keys[i]);
         __syncthreads();
     }
     if (wave) return;
     Sums t;
     uint32_t before = 0;
     for (uint32_t p = lane; p < a.pieces; p += 64) {
-        const float4 f = part[p];
+        const float4 f = p == lane ? first : part[p];
         Sums o;
         o.m = f.x;
         o.s = f.y;

@@ -553,25 +553,41 @@ def _refuse(cond, name: str, msg: str) -> None:
         raise NnzError(name, L.EINVAL, msg)
 
 
-def _is_rows(kv, t, rows: int, heads: int) -> bool:
-    """[rows, heads, head_dim] of the cache's type on its device, heads and dims
-    contiguous."""
-    return (t.dtype == kv.dtype and t.shape == (rows, heads, kv.head_dim) and t.stride(2) == 1
-            and (heads == 1 or t.stride(1) == kv.head_dim) and t.device == kv.device)
+def _rows_of(kv, t, rows: int, heads: int, name: str, what: str) -> int:
+    """Elements between the rows of t, which must be [rows, heads, head_dim] of
+    the cache's type on its device, heads and dims contiguous."""
+    d = kv.head_dim
+    if t.dtype is kv.dtype and t.device == kv.device and t.shape == (rows, heads, d):
+        between, head, one = t.stride()
+        if one == 1 and (head == d or heads == 1):
+            return between if rows > 1 else heads * d   # one row's stride says nothing
+    raise NnzError(name, L.EINVAL, what + " must be [num_rows, heads, head_dim] of the cache's type "
+                   "and device, heads and dims contiguous")
 
 
-def _is_flat(t, shape, types, device) -> bool:
-    """Absent, or contiguous of that shape, one of those types, on that device."""
-    return t is None or (t.shape == shape and str(t.dtype)[6:] in types and t.is_contiguous()
-                         and t.device == device)
+def _flat(t, shape, dtypes, device, name: str, what: str):
+    """The address of t, None if it is absent: contiguous, of that shape, one of
+    those types, on that device."""
+    if t is None:
+        return None
+    if t.dtype in dtypes and t.device == device and t.shape == shape and t.is_contiguous():
+        return t.data_ptr()
+    raise NnzError(name, L.EINVAL, f"{what} must be contiguous {tuple(shape)} of {dtypes} on {device}")
 
 
-_INT = ("int32", "uint32")
+class _Types:
+    """torch's types, named without importing torch here."""
+
+    def __getattr__(self, name):
+        t = _torch()
+        self.i32 = (t.int32, t.uint32)
+        self.f32 = (t.float32,)
+        self.f64 = (t.float64,)
+        self.logits = {t.float32: L.F32, t.float16: L.F16, t.bfloat16: L.BF16}
+        return self.__dict__[name]
 
 
-def _stride(t) -> int:
-    """Elements between rows; a single row's stride says nothing."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+_T = _Types()
 
 
 class PagedKVCache:
@@ -616,7 +632,7 @@ class PagedBatch:
                  max_kv_len: int):
         n = "PagedBatch"
         for t in (page_table, q_starts, kv_lens):
-            _refuse(str(t.dtype)[6:] not in _INT, n,
+            _refuse(t.dtype not in _T.i32, n,
                     "page_table, q_starts and kv_lens are 32-bit integers")
             _refuse(t.device != page_table.device, n,
                     "page_table, q_starts and kv_lens are on one device")
@@ -626,7 +642,7 @@ class PagedBatch:
         _refuse(q_starts.shape != (seqs + 1,) or kv_lens.shape != (seqs,), n,
                 "q_starts is [num_seqs + 1], kv_lens [num_seqs]")
         self.page_table, self.q_starts, self.kv_lens = page_table, q_starts, kv_lens
-        self.num_rows, self.num_seqs = num_rows, seqs
+        self.num_rows, self.num_seqs, self.device = num_rows, seqs, page_table.device
         self.desc = L.PagedBatchDesc(page_table.data_ptr(), q_starts.data_ptr(),
                                      kv_lens.data_ptr(), seqs, width, num_rows, max_q_len,
                                      max_kv_len, 0)
@@ -641,22 +657,16 @@ def dispatch_paged_append(dev, kv: PagedKVCache, batch: PagedBatch, q, k, v, q_o
     pages (transformer.zig:829 and :866 for many tokens).  Rows may be strided;
     rotary_dim defaults to D, inv_freq (f64) to theta^(-2k/rotary_dim)."""
     n, rows, d, hkv = "nnz_dispatch_paged_append", batch.num_rows, kv.head_dim, kv.num_kv_heads
-    hq = q.shape[1] if q.dim() == 3 else 0
-    _refuse(not (_is_rows(kv, q, rows, hq) and _is_rows(kv, q_out, rows, hq)), n,
-            "q and q_out are [num_rows, heads, head_dim] of the cache's type and device")
-    _refuse(not (_is_rows(kv, k, rows, hkv) and _is_rows(kv, v, rows, hkv)), n,
-            "k and v are [num_rows, num_kv_heads, head_dim] of the cache's type and device")
+    hq, at = q.shape[1] if q.dim() == 3 else 0, kv.device
+    _refuse(batch.device != at, n, "batch and cache are on two devices")
     rot = d if rotary_dim is None else rotary_dim
-    _refuse(not (_is_flat(q_scale, (d,), ("float32",), kv.device)
-                 and _is_flat(k_scale, (d,), ("float32",), kv.device)
-                 and _is_flat(inv_freq, (rot // 2,), ("float64",), kv.device)), n,
-            "norm scales are f32 [head_dim], inv_freq f64 [rotary_dim / 2], on the cache's device")
-    _refuse(batch.page_table.device != kv.device, n, "batch and cache are on two devices")
-    p = L.PagedAppendParams(_ptr(q_scale), _ptr(k_scale), _ptr(inv_freq), hq, _stride(q),
-                            _stride(k), _stride(v), _stride(q_out), rot, int(halves), theta, eps,
-                            0)
-    dev.call(n, kv.ref, batch.ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(),
-             C.byref(p))
+    p = L.PagedAppendParams(_flat(q_scale, (d,), _T.f32, at, n, "q_scale"),
+                            _flat(k_scale, (d,), _T.f32, at, n, "k_scale"),
+                            _flat(inv_freq, (rot // 2,), _T.f64, at, n, "inv_freq"), hq,
+                            _rows_of(kv, q, rows, hq, n, "q"), _rows_of(kv, k, rows, hkv, n, "k"),
+                            _rows_of(kv, v, rows, hkv, n, "v"),
+                            _rows_of(kv, q_out, rows, hq, n, "q_out"), rot, halves, theta, eps)
+    dev.call(n, kv.ref, batch.ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(), p)
 
 
 def paged_attention_workspace_bytes(kv: PagedKVCache, batch: PagedBatch,
@@ -671,21 +681,16 @@ def dispatch_paged_attention(dev, kv: PagedKVCache, batch: PagedBatch, q, out, w
     (chunks of prompts and single tokens alike) -> out, and optionally lse f32
     [rows, Hq].  softcap caps the scores, slopes f32 [Hq] biases them by
     distance, window and prefix_lens int32 [num_seqs] shape the mask."""
-    n, rows = "nnz_dispatch_paged_attention", batch.num_rows
+    n, rows, at = "nnz_dispatch_paged_attention", batch.num_rows, kv.device
     hq = q.shape[1] if q.dim() == 3 else 0
-    _refuse(not (_is_rows(kv, q, rows, hq) and _is_rows(kv, out, rows, hq)), n,
-            "q and out are [num_rows, heads, head_dim] of the cache's type and device")
-    _refuse(not (_is_flat(lse, (rows, hq), ("float32",), kv.device)
-                 and _is_flat(slopes, (hq,), ("float32",), kv.device)
-                 and _is_flat(prefix_lens, (batch.num_seqs,), _INT, kv.device)), n,
-            "lse is f32 [num_rows, heads], slopes f32 [heads], prefix_lens int32 [num_seqs], "
-            "on the cache's device")
-    _refuse(batch.page_table.device != kv.device, n, "batch and cache are on two devices")
-    p = L.PagedAttnParams(_ptr(slopes), _ptr(prefix_lens), hq, _stride(q), _stride(out), window,
-                          scale, softcap)
-    dev.call(n, kv.ref, batch.ref, q.data_ptr(), out.data_ptr(), _ptr(lse), _ptr(workspace),
-             workspace.numel() * workspace.element_size() if workspace is not None else 0,
-             C.byref(p))
+    _refuse(batch.device != at, n, "batch and cache are on two devices")
+    p = L.PagedAttnParams(_flat(slopes, (hq,), _T.f32, at, n, "slopes"),
+                          _flat(prefix_lens, (batch.num_seqs,), _T.i32, at, n, "prefix_lens"), hq,
+                          _rows_of(kv, q, rows, hq, n, "q"), _rows_of(kv, out, rows, hq, n, "out"),
+                          window, scale, softcap)
+    dev.call(n, kv.ref, batch.ref, q.data_ptr(), out.data_ptr(),
+             _flat(lse, (rows, hq), _T.f32, at, n, "lse"), _ptr(workspace),
+             0 if workspace is None else workspace.nbytes, p)
 
 
 def token_logprobs_workspace_bytes(rows: int, vocab: int, top_n: int = 0) -> int:
@@ -698,26 +703,22 @@ def dispatch_token_logprobs(dev, logits, tokens, logprobs, workspace, lse=None, 
     with the row's lse, entropy, the token's rank and the best alternatives (as
     many as top_ids / top_logprobs have columns).  logits [rows, vocab] f32, f16
     or bf16, rows may be strided; integers are int32."""
-    n = "nnz_dispatch_token_logprobs"
-    _refuse(logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1), n,
-            "logits are [rows, vocab] with contiguous rows")
-    _refuse(str(logits.dtype)[6:] not in _DT, n, "logits are f32, f16 or bf16")
+    n, at = "nnz_dispatch_token_logprobs", logits.device
+    kind = _T.logits.get(logits.dtype)
+    _refuse(logits.dim() != 2 or kind is None or at != dev.torch_device, n,
+            "logits are [rows, vocab] in f32, f16 or bf16 on the context's device")
     rows, vocab = logits.shape
+    between, one = logits.stride()
+    _refuse(vocab > 1 and one != 1, n, "rows of logits must be contiguous")
     top = next((t.shape[1] for t in (top_ids, top_logprobs) if t is not None and t.dim() == 2), 0)
-    one, table, f, at = (rows,), (rows, top), ("float32",), logits.device
-    _refuse(not (_is_flat(tokens, one, _INT, at) and _is_flat(logprobs, one, f, at)
-                 and _is_flat(lse, one, f, at) and _is_flat(entropy, one, f, at)
-                 and _is_flat(rank, one, _INT, at) and _is_flat(top_ids, table, _INT, at)
-                 and _is_flat(top_logprobs, table, f, at)), n,
-            "tokens, rank and top_ids are int32, the rest f32; [rows] or [rows, top_n], contiguous, "
-            "on the logits' device")
-    _refuse(at != dev.torch_device, n, "logits are not on the context's device")
-    stride = logits.stride(0) if rows > 1 else vocab
-    d = L.LogprobsDims(stride, rows, vocab, top, dtype_code(logits), temperature, 0)
-    dev.call(n, logits.data_ptr(), _ptr(tokens), _ptr(logprobs), _ptr(lse), _ptr(entropy),
-             _ptr(rank), _ptr(top_ids), _ptr(top_logprobs), _ptr(workspace),
-             workspace.numel() * workspace.element_size() if workspace is not None else 0,
-             C.byref(d))
+    row, table = (rows,), (rows, top)
+    d = L.LogprobsDims(between if rows > 1 else vocab, rows, vocab, top, kind, temperature)
+    dev.call(n, logits.data_ptr(), _flat(tokens, row, _T.i32, at, n, "tokens"),
+             _flat(logprobs, row, _T.f32, at, n, "logprobs"), _flat(lse, row, _T.f32, at, n, "lse"),
+             _flat(entropy, row, _T.f32, at, n, "entropy"), _flat(rank, row, _T.i32, at, n, "rank"),
+             _flat(top_ids, table, _T.i32, at, n, "top_ids"),
+             _flat(top_logprobs, table, _T.f32, at, n, "top_logprobs"), _ptr(workspace),
+             0 if workspace is None else workspace.nbytes, d)
 
 
 __all__ = [n for n in dir() if n.startswith("dispatch_")] + ["Device", "DeviceQWeight",
