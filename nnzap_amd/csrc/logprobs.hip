@@ -11,8 +11,8 @@
 //   * the number of ids that come before the token, counted from the compares'
 //     lane masks;
 //   * candidates for the best top_n.  A group of 16 values per lane is looked at
-//     again only if one of them reaches the wave's bound; the bound rises to a
-//     value that top_n of the lanes' maxima reach (top_n values of the row are
+//     again only if one of them reaches the bound; a wave's bound, which serves
+//     the whole block, rises to a value that top_n of the lanes' maxima reach (top_n values of the row are
 //     no smaller: 12 ballots find sign, exponent and three bits), and what reaches it waits in
 //     LDS with its id.  Should more than 128 wait, they are sorted, 64 at a
 //     time, into a list of keys (value and complemented id: larger is earlier),
@@ -170,7 +170,7 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LpArgs a) {
     constexpr uint32_t ESZ = DT == NNZ_F32 ? 4 : 2, VE = 16 / ESZ, U = GROUP / VE;   // values of a vector, vectors of a group
     __shared__ uint2 pool[WAVES][WAITING + 64 * GROUP + 64];   // value and id; later keys
     __shared__ float4 sums[WAVES];
-    __shared__ float bounds[WAVES];
+    __shared__ float bounds[WAVES];   // the waves' bounds, as they rise
     __shared__ uint32_t counts[WAVES];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t row = blockIdx.x / a.pieces, piece = blockIdx.x % a.pieces;
@@ -195,11 +195,16 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LpArgs a) {
     const bool named = tok < a.vocab, order = named && a.rank;
     const float xt = named ? load_as_f32<DT>(base, tok) : 0.f;
 
+    if (threadIdx.x < WAVES) bounds[threadIdx.x] = -INFINITY;
+    __syncthreads();
     Sums t;
     uint32_t before = 0, held = 0;   // held: candidates waiting in the pool
     uint64_t list = 0;
     float bound = -INFINITY;         // what a candidate reaches, or, with `above`, passes
     bool above = false;
+    auto tell = [&]() __attribute__((always_inline)) {
+        if (lane == 0) __hip_atomic_store(&bounds[wave], bound, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    };
     auto settle = [&]() __attribute__((always_inline)) {   // LDS written by this wave is there for it
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -218,9 +223,10 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LpArgs a) {
         }
         held = 0;
         const uint64_t last = lane_key(list, a.top - 1);
-        if (last) {
+        if (last && key_value(last) >= bound) {
             bound = key_value(last);
             above = true;
+            tell();
         }
     };
     // n values of a lane (at most GROUP), ids id(e); those with !on(e) are not there
@@ -252,20 +258,41 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LpArgs a) {
                     add(on(e) && (xt != xt ? x[e] == x[e] || id(e) < tok : x[e] > xt || (x[e] == xt && id(e) < tok)));
             }
         }
-        if (a.top && __builtin_amdgcn_ballot_w64(above ? mx > bound : mx >= bound)) {
-            const float to = reached_by(mx, a.top);
-            if (to > bound) {
-                bound = to;
-                above = false;
+        if (!a.top) return;
+        // any wave's bound is one of the block's
+        float others = -INFINITY;
+#pragma unroll
+        for (uint32_t i = 0; i < WAVES; ++i)
+            others = fmaxf(others, __hip_atomic_load(&bounds[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP));
+        if (others > bound) {
+            bound = others;
+            above = false;
+        }
+        const uint64_t reach = __builtin_amdgcn_ballot_w64(above ? mx > bound : mx >= bound);
+        if (reach) {
+            if (__builtin_popcountll(reach) >= (int)a.top) {   // else it cannot rise
+                const float to = reached_by(mx, a.top);
+                if (to > bound) {
+                    bound = to;
+                    above = false;
+                    tell();
+                }
             }
 #pragma unroll
-            for (uint32_t e = 0; e < n; ++e) {
-                const bool mine = on(e) && (above ? x[e] > bound : x[e] >= bound);
-                const uint64_t in = __builtin_amdgcn_ballot_w64(mine);
-                if (in) {
-                    const uint32_t at = __builtin_amdgcn_mbcnt_hi((uint32_t)(in >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in, 0));
-                    if (mine) pool[wave][held + at] = make_uint2(__float_as_uint(x[e]), id(e));
-                    held += __builtin_popcountll(in);
+            for (uint32_t q = 0; q < n; q += 4) {
+                float m4 = x[q];
+#pragma unroll
+                for (uint32_t e = q + 1; e < q + 4 && e < n; ++e) m4 = fmaxf(m4, x[e]);
+                if (!__builtin_amdgcn_ballot_w64(m4 >= bound)) continue;
+#pragma unroll
+                for (uint32_t e = q; e < q + 4 && e < n; ++e) {
+                    const bool mine = on(e) && (above ? x[e] > bound : x[e] >= bound);
+                    const uint64_t in = __builtin_amdgcn_ballot_w64(mine);
+                    if (in) {
+                        const uint32_t at = __builtin_amdgcn_mbcnt_hi((uint32_t)(in >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in, 0));
+                        if (mine) pool[wave][held + at] = make_uint2(__float_as_uint(x[e]), id(e));
+                        held += __builtin_popcountll(in);
+                    }
                 }
             }
             if (held > WAITING) drain();

@@ -438,7 +438,7 @@ def _check_logprobs(x, tok, got, top, T=1.0):
 
 
 SIZES = [(1, 1), (3, 2), (2, 5), (4, 63), (3, 64), (5, 65), (2, 255), (7, 1000), (3, 4097), (2, 50257), (1, 151669),
-         (90, 3001)]
+         (90, 3001), (300, 17_001)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, F16, BF16])
@@ -499,14 +499,14 @@ def test_logprobs_of_far_rows(dev):
 
 
 def test_logprobs_refuses_a_short_workspace(dev):
-    x, tok = torch.randn(1, 151_669, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
-    n = ops.token_logprobs_workspace_bytes(1, 151_669, 20)
+    x, tok = torch.randn(300, 20_000, device="cuda"), torch.zeros(300, dtype=torch.int32, device="cuda")
+    n = ops.token_logprobs_workspace_bytes(300, 20_000, 20)
     assert n > 0
-    ids = torch.zeros(1, 20, dtype=torch.int32, device="cuda")
+    ids = torch.zeros(300, 20, dtype=torch.int32, device="cuda")
     for ws in (None, torch.zeros(n - 1, dtype=torch.uint8, device="cuda"),
                torch.zeros(n + 16, dtype=torch.uint8, device="cuda")[8:]):
         with pytest.raises(NnzError, match="workspace"):
-            ops.dispatch_token_logprobs(dev, x, tok, torch.zeros(1, device="cuda"), ws, top_ids=ids)
+            ops.dispatch_token_logprobs(dev, x, tok, torch.zeros(300, device="cuda"), ws, top_ids=ids)
 
 
 # ------------------------------------------------- used together, as a server does
