@@ -10,16 +10,19 @@
 //     log s - w / s is a sum of terms of one sign;
 //   * the number of ids that come before the token, counted from the compares'
 //     lane masks;
-//   * candidates for the best top_n.  A group of 16 values per lane is looked at
-//     again only if one of them reaches the bound; a wave's bound, which serves
-//     the whole block, rises to a value that top_n of the lanes' maxima reach (top_n values of the row are
-//     no smaller: 12 ballots find sign, exponent and three bits), and what reaches it waits in
-//     LDS with its id.  Should more than 128 wait, they are sorted, 64 at a
-//     time, into a list of keys (value and complemented id: larger is earlier),
+//   * candidates for the best top_n, which wait in LDS with their ids.  A group of
+//     16 values per lane is looked at again only if one of them reaches the bound,
+//     a value that top_n values of the block's part are known to reach: the
+//     top_n-th largest of a wave's lane maxima (16 ballots find its upper half).
+//     When more than 48 + top_n wait, the same over them raises the bound and
+//     leaves about top_n.  Where values are equal it leaves too many: they are
+//     sorted into a list of keys (value and complemented id: larger is earlier),
 //     whose last bounds what follows.  Ids rise along a wave's part, so that a
 //     full list lets no equal value in: rows of equal values cost one list.
 // At the end the largest of the waves' bounds leaves a few dozen of the block's
 // candidates, which one sort puts in order; the pieces' lists likewise.
+// Measured: 2048 x 151936 f32 193 us (6.4 TB/s), one row of 151669 14 us, of it 4
+// the join; the candidates cost calls of few rows most (one row without: 11 us).
 // Keys and counts are integers and the partial sums meet in a fixed order, so a
 // call repeats bit for bit.
 #include "paged_dev.h"
@@ -31,7 +34,7 @@ namespace {
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 
 constexpr uint32_t WAVES = 4, GROUP = 16;   // values of a lane looked at together
-constexpr uint32_t WAITING = 128;           // candidates of a wave that may stay unsorted
+constexpr uint32_t WAITING = 112;           // most candidates of a wave that wait (48 + top)
 constexpr float LN2 = 0.69314718055994531f, LOG2E = 1.44269504088896341f;
 
 struct LpArgs {
@@ -131,17 +134,65 @@ struct Sums {
     }
 };
 
-// A value that at least n lanes' x reach, at most an eighth below the n-th
-// largest of them.
-__device__ __forceinline__ float reached_by(float x, uint32_t n) {
-    const uint32_t u = __float_as_uint(x + 0.f), k = u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+// The upper half of order_key, and back.
+__device__ __forceinline__ uint32_t order_of(float x) {
+    const uint32_t u = __float_as_uint(x + 0.f);
+    return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float value_of(uint32_t m) {   // what lies below -inf counts as it
+    return m <= 0x007FFFFFu ? -INFINITY : __uint_as_float(m >> 31 ? m & 0x7fffffffu : ~m);
+}
+// The n-th largest of the lanes' values, its lower 16 bits cleared: n of them
+// reach it.
+__device__ __forceinline__ uint32_t reached_by(uint32_t k, uint32_t n) {
     uint32_t f = 0;
 #pragma unroll
-    for (int b = 31; b >= 20; --b) {
+    for (int b = 31; b >= 16; --b) {
         const uint32_t up = f | 1u << b;
         f = __builtin_popcountll(__builtin_amdgcn_ballot_w64(k >= up)) >= (int)n ? up : f;
     }
-    return f <= 0x007FFFFFu ? -INFINITY : __uint_as_float(f >> 31 ? f & 0x7fffffffu : ~f);
+    return f;
+}
+__device__ __forceinline__ uint32_t lanes_below(uint64_t mask) {
+    return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+}
+
+// The 64 largest of n keys, falling, by one wave.  More than 64 are first cut to
+// those that reach what `top` of the lanes' largest do, by way of `room` in LDS (up
+// to 640 of them); where many are equal, 64 at a time are sorted and merged.
+template <class Key>
+__device__ __forceinline__ uint64_t sort_some(uint32_t n, uint32_t top, Key key_at, uint64_t *room) {
+    const uint32_t lane = threadIdx.x & 63;
+    bool moved = false;
+    if (n > 64 && n <= 640) {
+        uint32_t k = 0;
+        for (uint32_t j = lane; j < n; j += 64) {
+            const uint32_t m = (uint32_t)(key_at(j) >> 32);
+            k = m > k ? m : k;
+        }
+        const uint32_t f = reached_by(k, top);
+        uint32_t kept = 0;
+        for (uint32_t j = 0; j < n; j += 64) {
+            const uint64_t v = j + lane < n ? key_at(j + lane) : 0;
+            const uint64_t in = __builtin_amdgcn_ballot_w64(v != 0 && (uint32_t)(v >> 32) >= f);
+            if (in >> lane & 1) room[kept + lanes_below(in)] = v;
+            kept += __builtin_popcountll(in);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        n = kept;
+        moved = true;
+    }
+    uint64_t list = 0;
+    for (uint32_t j = 0; j < n; j += 64) {
+        uint64_t k = sort64(j + lane < n ? (moved ? room[j + lane] : key_at(j + lane)) : 0);
+        if (j) {   // two falling lists: the second one backwards
+            const uint32_t lo = __shfl((uint32_t)k, 63 - lane), hi = __shfl((uint32_t)(k >> 32), 63 - lane);
+            k = merge64(list, (uint64_t)hi << 32 | lo);
+        }
+        list = k;
+    }
+    return list;
 }
 
 // Row-wide results, by one wave: its sums, count and list (lane i holds the
@@ -197,6 +248,7 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LpArgs a) {
 
     if (threadIdx.x < WAVES) bounds[threadIdx.x] = -INFINITY;
     __syncthreads();
+    const uint32_t waiting = 48 + a.top;
     Sums t;
     uint32_t before = 0, held = 0;   // held: candidates waiting in the pool
     uint64_t list = 0;
@@ -209,8 +261,37 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LpArgs a) {
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
     };
-    auto drain = [&]() __attribute__((always_inline)) {   // the pool joins the list
+    // Raises the bound to what top of the lanes' largest candidates reach, and
+    // leaves the candidates that do.
+    auto narrow = [&]() __attribute__((always_inline)) {
         settle();
+        uint32_t k = 0;
+        for (uint32_t at = 0; at < held; at += 64) {
+            const uint32_t m = order_of(__uint_as_float(pool[wave][at + lane].x));
+            k = at + lane < held && m > k ? m : k;
+        }
+        const float to = value_of(reached_by(k, a.top));
+        if (to > bound) {
+            bound = to;
+            above = false;
+            tell();
+        }
+        uint32_t kept = 0;
+        for (uint32_t at = 0; at < held; at += 64) {
+            const uint2 f = pool[wave][at + lane];
+            const uint64_t in = __builtin_amdgcn_ballot_w64(at + lane < held && __uint_as_float(f.x) >= bound);
+            settle();
+            if (in >> lane & 1) pool[wave][kept + lanes_below(in)] = f;
+            settle();
+            kept += __builtin_popcountll(in);
+        }
+        held = kept;
+    };
+    // Where values are equal that leaves too many: sorted into a list of keys,
+    // whose last id bounds them too.
+    auto drain = [&]() __attribute__((always_inline)) {
+        narrow();
+        if (held <= waiting) return;
         for (uint32_t at = 0; at < held; at += 64) {
             const uint2 f = pool[wave][at + lane];
             const uint64_t k = sort64(at + lane < held ? order_key(__uint_as_float(f.x), f.y) : 0);
@@ -271,7 +352,7 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LpArgs a) {
         const uint64_t reach = __builtin_amdgcn_ballot_w64(above ? mx > bound : mx >= bound);
         if (reach) {
             if (__builtin_popcountll(reach) >= (int)a.top) {   // else it cannot rise
-                const float to = reached_by(mx, a.top);
+                const float to = value_of(reached_by(order_of(mx), a.top));
                 if (to > bound) {
                     bound = to;
                     above = false;
@@ -289,13 +370,12 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LpArgs a) {
                     const bool mine = on(e) && (above ? x[e] > bound : x[e] >= bound);
                     const uint64_t in = __builtin_amdgcn_ballot_w64(mine);
                     if (in) {
-                        const uint32_t at = __builtin_amdgcn_mbcnt_hi((uint32_t)(in >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in, 0));
-                        if (mine) pool[wave][held + at] = make_uint2(__float_as_uint(x[e]), id(e));
+                        if (mine) pool[wave][held + lanes_below(in)] = make_uint2(__float_as_uint(x[e]), id(e));
                         held += __builtin_popcountll(in);
                     }
                 }
             }
-            if (held > WAITING) drain();
+            if (held > waiting) drain();
         }
     };
     auto unpack = [&](const v4u (&r)[U], float *x) __attribute__((always_inline)) {
@@ -341,6 +421,7 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LpArgs a) {
     }
 
     // the wave's lanes, then the block's waves
+    if (held > a.top) narrow();
     t.join_lanes(a.c);
     if (lane == 0) {
         sums[wave] = make_float4(t.m, t.s, t.w, __uint_as_float(before));
@@ -353,9 +434,8 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LpArgs a) {
         uint32_t kept = 0;
         auto put = [&](uint64_t k) __attribute__((always_inline)) {
             const uint64_t in = __builtin_amdgcn_ballot_w64(k != 0);
-            const uint32_t at = __builtin_amdgcn_mbcnt_hi((uint32_t)(in >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in, 0));
             settle();
-            if (k) pool[wave][kept + at] = make_uint2((uint32_t)k, (uint32_t)(k >> 32));
+            if (k) pool[wave][kept + lanes_below(in)] = make_uint2((uint32_t)k, (uint32_t)(k >> 32));
             settle();
             kept += __builtin_popcountll(in);
         };
@@ -380,18 +460,13 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LpArgs a) {
         before += __float_as_uint(f.w);
     }
     if (a.top) {
-        const uint32_t n0 = counts[0], n1 = n0 + counts[1], n2 = n1 + counts[2], n3 = n2 + counts[3];
-        list = 0;
-        for (uint32_t j = 0; j < n3; j += 64) {
-            const uint32_t i = j + lane;
-            const uint2 f = i < n0 ? pool[0][i] : i < n1 ? pool[1][i - n0] : i < n2 ? pool[2][i - n1] : pool[3][i < n3 ? i - n2 : 0];
-            uint64_t k = sort64(i < n3 ? (uint64_t)f.y << 32 | f.x : 0);
-            if (j) {   // two falling lists: the second one backwards
-                const uint32_t lo = __shfl((uint32_t)k, 63 - lane), hi = __shfl((uint32_t)(k >> 32), 63 - lane);
-                k = merge64(list, (uint64_t)hi << 32 | lo);
-            }
-            list = k;
-        }
+        const uint32_t n0 = counts[0], n1 = n0 + counts[1], n2 = n1 + counts[2];
+        uint32_t n = n2 + counts[3];
+        auto key_at = [&](uint32_t i) {
+            const uint2 f = i < n0 ? pool[0][i] : i < n1 ? pool[1][i - n0] : i < n2 ? pool[2][i - n1] : pool[3][i < n ? i - n2 : 0];
+            return i < n ? (uint64_t)f.y << 32 | f.x : 0;
+        };
+        list = sort_some(n, a.top, key_at, (uint64_t *)&pool[0][2 * WAITING]);
     }
     if (a.pieces == 1) {
         finish(a, row, t, before, list, xt, named);
@@ -408,8 +483,8 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LpArgs a) {
 template <int DT>
 __global__ __launch_bounds__(256) void logprobs_join_kernel(LpArgs a) {
     extern __shared__ uint64_t kept[];   // [pieces * top]
-    __shared__ uint64_t reach[WAVES];
-    __shared__ uint32_t count;
+    __shared__ uint64_t reach[WAVES], room[640];
+    __shared__ uint32_t most[WAVES], count;
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), row = blockIdx.x;
     const float4 *const part = a.part + (size_t)row * a.pieces;
     const uint64_t *const keys = a.part_keys + (size_t)row * a.pieces * a.top;
@@ -432,9 +507,19 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(LpArgs a) {
         }
         if (lane == 0) reach[wave] = k;
         if (tid == 0) count = 0;
+        // and what top of a wave's lanes reach
+        uint32_t m = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) m = (uint32_t)(mine[i] >> 32) > m ? (uint32_t)(mine[i] >> 32) : m;
+        m = reached_by(m, a.top);
+        if (lane == 0) most[wave] = m;
         __syncthreads();
 #pragma unroll
-        for (uint32_t i = 0; i < WAVES; ++i) k = reach[i] > k ? reach[i] : k;
+        for (uint32_t i = 0; i < 4; ++i) {
+            k = reach[i] > k ? reach[i] : k;
+            m = most[i] > m ? most[i] : m;
+        }
+        k = (uint64_t)m << 32 > k ? (uint64_t)m << 32 : k;
         auto put = [&](uint64_t v) {
             if (v && v >= k) kept[atomicAdd(&count, 1u)] = v;   // any order: they are sorted next
         };
@@ -458,16 +543,7 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(LpArgs a) {
     t.join_lanes(a.c);
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) before += __shfl_xor(before, o);
-    uint64_t list = 0;
-    if (a.top)
-        for (uint32_t j = 0; j < count; j += 64) {
-            uint64_t k = sort64(j + lane < count ? kept[j + lane] : 0);
-            if (j) {
-                const uint32_t lo = __shfl((uint32_t)k, 63 - lane), hi = __shfl((uint32_t)(k >> 32), 63 - lane);
-                k = merge64(list, (uint64_t)hi << 32 | lo);
-            }
-            list = k;
-        }
+    const uint64_t list = a.top ? sort_some(count, a.top, [&](uint32_t i) { return kept[i]; }, room) : 0;
     finish(a, row, t, before, list, xt, named);
 }
 
