@@ -27,6 +27,9 @@ typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 // stay within 16 (8 at head_dim 64) lanes, with the group's cosines and sines
 // computed once into LDS.  V goes to its transposed page two dims a lane, all
 // positions of the group in registers: whole groups are two 16-byte stores.
+// q and k leave past the caches: 8192 tokens of 32 + 8 heads 60 -> 55 us (201 MB,
+// 3.7 TB/s), 4093 tokens of seven prompts 31 -> 26 us; V's 16-byte pieces not,
+// they meet in the L2 (past it: 70 us).
 template <int D, bool BF>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     constexpr uint32_t LPR = D / 8, SETS = 256 / LPR;   // lanes of a row, rows at a time
@@ -143,7 +146,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
         if (on) {
             uint16_t *dst = h < a.hq ? a.q_out + row * a.qo_stride + h * D
                                      : a.k_pages + (((((size_t)page * a.b.hkv + h - a.hq) << a.b.shift) + slot + tok) * D);
-            *(v4u *)(dst + d0) = y;
+            __builtin_nontemporal_store(y, (v4u *)(dst + d0));
         }
         r = next;
     }
@@ -152,12 +155,13 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
 template <int D, bool BF>
 int launch(nnz_ctx *ctx, const AppendArgs &a) {
     // Groups of 8 positions, an upper bound; the heads are shared out until
-    // there are about 1024 blocks, down to four rows of heads for a thread (one
-    // for single tokens, whose blocks take 16 heads at a time).
+    // there are about 4096 blocks, down to four rows of heads for a thread (one
+    // for single tokens, whose blocks take 16 heads at a time).  1024 blocks:
+    // 8192 tokens of 32 + 8 heads 65 us against 60.
     const uint64_t groups = std::min<uint64_t>((uint64_t)a.b.rows / 8 + 2ull * a.b.num_seqs,
                                                (uint64_t)a.b.num_seqs * paged_groups_max(a.b.max_q));
     const uint32_t heads = a.hq + a.b.hkv, most = ceil_div(heads, a.b.max_q > 1 ? 8 : 16);
-    const uint32_t shares = std::min(most, (uint32_t)std::max<uint64_t>(1, 1024 / groups));
+    const uint32_t shares = std::min(most, (uint32_t)std::max<uint64_t>(1, 4096 / groups));
     append_kernel<D, BF><<<dim3((uint32_t)groups, shares), 256, 0, ctx->stream>>>(a);
     NNZ_LAUNCHED(ctx);
     return NNZ_OK;
