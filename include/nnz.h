@@ -584,8 +584,8 @@ typedef struct {
     uint32_t num_query_heads;     /* a multiple of num_kv_heads */
     uint32_t q_stride, out_stride;/* elements between rows, multiples of 8 */
     uint32_t window;              /* 0: no window */
-    float scale;                  /* > 0, or 0: 1 / sqrt(head_dim) */
-    float softcap;                /* > 0, or 0: not capped */
+    float scale;                  /* 1e-30 to 1e30, or 0: 1 / sqrt(head_dim) */
+    float softcap;                /* 1e-6 to 1e6, or 0: not capped */
 } nnz_paged_attn_params;
 size_t nnz_paged_attention_workspace_bytes(const nnz_paged_kv *kv, const nnz_paged_batch *batch,
                                            uint32_t num_query_heads);
@@ -616,7 +616,7 @@ int nnz_dispatch_paged_attention(nnz_ctx *ctx, const nnz_paged_kv *kv,
 typedef struct {
     uint64_t row_stride;          /* elements between rows, >= vocab */
     uint32_t rows, vocab, top_n, dtype;
-    float temperature;            /* > 0 */
+    float temperature;            /* 1e-30 to 1e30 */
     uint32_t reserved;            /* unused */
 } nnz_logprobs_dims;
 size_t nnz_token_logprobs_workspace_bytes(uint32_t rows, uint32_t vocab, uint32_t top_n);

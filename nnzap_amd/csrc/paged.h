@@ -162,8 +162,11 @@ inline PagedFault paged_attn_fault(const nnz_paged_kv *kv, const nnz_paged_batch
     if (PagedFault f = paged_rows_fault(q, p->q_stride, p->num_query_heads, kv->head_dim); f.code) return f;
     if (PagedFault f = paged_rows_fault(out, p->out_stride, p->num_query_heads, kv->head_dim); f.code) return f;
     if (q == out) return {NNZ_EINVAL, "the output may not overwrite q"};
-    if (!(p->scale >= 0.f && p->scale < 3e38f)) return {NNZ_EINVAL, "scale must be positive, or 0 for 1/sqrt(head_dim)"};
-    if (!(p->softcap >= 0.f && p->softcap < 3e38f)) return {NNZ_EINVAL, "softcap must be positive, or 0 for none"};
+    // beyond these what the kernels derive from them leaves float32
+    if (p->scale != 0.f && !(p->scale >= 1e-30f && p->scale <= 1e30f))
+        return {NNZ_EINVAL, "scale must be from 1e-30 to 1e30, or 0 for 1/sqrt(head_dim)"};
+    if (p->softcap != 0.f && !(p->softcap >= 1e-6f && p->softcap <= 1e6f))
+        return {NNZ_EINVAL, "softcap must be from 1e-6 to 1e6, or 0 for none"};
     if (((uintptr_t)lse | (uintptr_t)p->slopes | (uintptr_t)p->prefix_lens) & 3)
         return {NNZ_EINVAL, "lse, slopes and prefix_lens must be 4-byte aligned"};
     return {NNZ_OK, nullptr};
@@ -173,13 +176,13 @@ inline PagedFault logprobs_fault(const void *logits, const uint32_t *tokens, con
                                  const uint32_t *top_ids, const float *top_logprobs, const nnz_logprobs_dims *d) {
     if (!d || !logits || !tokens || !logprobs) return {NNZ_EINVAL, "null dims, logits, tokens or logprobs"};
     if (d->dtype != NNZ_F32 && d->dtype != NNZ_F16 && d->dtype != NNZ_BF16) return {NNZ_EINVAL, "bad dtype"};
-    if (!d->rows || d->rows > (1u << 24)) return {NNZ_EINVAL, "rows is 1 to 2^24"};
+    if (!d->rows || d->rows >= (1u << 24)) return {NNZ_EINVAL, "rows is 1 to 2^24 - 1"};
     if (!d->vocab || d->vocab > (1u << 28)) return {NNZ_EINVAL, "vocab is 1 to 2^28"};
     if (d->row_stride < d->vocab) return {NNZ_EINVAL, "row_stride is less than vocab"};
     if (d->row_stride > (1ull << 32)) return {NNZ_EINVAL, "row_stride out of range"};
     if (d->top_n > 64 || d->top_n > d->vocab) return {NNZ_EINVAL, "top_n is at most 64 and vocab"};
     if (d->top_n && !(top_ids || top_logprobs)) return {NNZ_EINVAL, "top_n without top_ids and top_logprobs"};
-    if (!(d->temperature > 0.f && d->temperature < 3e38f)) return {NNZ_EINVAL, "temperature must be positive"};
+    if (!(d->temperature >= 1e-30f && d->temperature <= 1e30f)) return {NNZ_EINVAL, "temperature must be from 1e-30 to 1e30"};
     if ((uintptr_t)logits & (d->dtype == NNZ_F32 ? 3 : 1)) return {NNZ_EINVAL, "logits are not aligned to their type"};
     return {NNZ_OK, nullptr};
 }

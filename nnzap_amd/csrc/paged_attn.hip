@@ -653,8 +653,8 @@ __device__ __forceinline__ void chunk_part(const AttnArgs &a, uint32_t block, Ch
     const float2 lp = swap32(l, l);
     l = lp.x + lp.y;
     float M = m == -INFINITY ? -INFINITY : -nm;
-    if (lane == 0) sh.odd[group][wave] = 0;
-    if (odd) sh.odd[group][wave] = 1;   // after the store above, both by this wave
+    const bool met = __builtin_amdgcn_ballot_w64(odd != 0) != 0;
+    if (lane == 0) sh.odd[group][wave] = met;
     __syncthreads();
     if (__builtin_expect(sh.odd[group][0] | sh.odd[group][1] | sh.odd[group][2] | sh.odd[group][3], 0)) {   // group-uniform
         for (uint32_t t = ta; t < t1; t += 2) {
@@ -947,8 +947,8 @@ extern "C" int nnz_dispatch_paged_attention(nnz_ctx *ctx, const nnz_paged_kv *kv
         return nnz_fail(ctx, f.code, "paged_attention: %s", f.what);
     const Plan plan = plan_of(*kv, *batch, p->num_query_heads);
     const size_t need = bytes_of(plan, kv->head_dim);
-    NNZ_REQUIRE(ctx, blocks_of(plan, *batch, kv->num_kv_heads) < (1u << 24), NNZ_EUNSUPPORTED,
-                "paged_attention: more than 2^24 blocks; split the batch");
+    NNZ_REQUIRE(ctx, blocks_of(plan, *batch, kv->num_kv_heads) < (1u << 23), NNZ_EUNSUPPORTED,
+                "paged_attention: more than 2^23 blocks; split the batch");
     NNZ_REQUIRE(ctx, need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0), NNZ_EINVAL,
                 "paged_attention: workspace of %zu bytes, 16-byte aligned, needed (%zu given)", need, workspace_bytes);
     NnzDeviceScope scope(ctx);

@@ -684,6 +684,7 @@ def dispatch_paged_attention(dev, kv: PagedKVCache, batch: PagedBatch, q, out, w
     n, rows, at = "nnz_dispatch_paged_attention", batch.num_rows, kv.device
     hq = q.shape[1] if q.dim() == 3 else 0
     _refuse(batch.device != at, n, "batch and cache are on two devices")
+    _refuse(window < 0, n, "window must not be negative")
     p = L.PagedAttnParams(_flat(slopes, (hq,), _T.f32, at, n, "slopes"),
                           _flat(prefix_lens, (batch.num_seqs,), _T.i32, at, n, "prefix_lens"), hq,
                           _rows_of(kv, q, rows, hq, n, "q"), _rows_of(kv, out, rows, hq, n, "out"),

@@ -2,6 +2,13 @@
 // (nnzap_amd/csrc/paged.h), exported for tests/test_serving_host.py.
 #include "../../nnzap_amd/csrc/paged.h"
 
+// the layouts that nnzap_amd/_lib.py states
+static_assert(sizeof(nnz_paged_kv) == 40 && offsetof(nnz_paged_kv, dtype) == 32, "nnz_paged_kv");
+static_assert(sizeof(nnz_paged_batch) == 48 && offsetof(nnz_paged_batch, max_kv_len) == 40, "nnz_paged_batch");
+static_assert(sizeof(nnz_paged_append_params) == 64 && offsetof(nnz_paged_append_params, eps) == 56, "nnz_paged_append_params");
+static_assert(sizeof(nnz_paged_attn_params) == 40 && offsetof(nnz_paged_attn_params, softcap) == 36, "nnz_paged_attn_params");
+static_assert(sizeof(nnz_logprobs_dims) == 32 && offsetof(nnz_logprobs_dims, temperature) == 24, "nnz_logprobs_dims");
+
 extern "C" {
 
 static int tell(PagedFault f, const char **what) {

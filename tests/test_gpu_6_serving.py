@@ -297,6 +297,78 @@ def test_large_scores(dev):
         _check_attention(c, kp, vp, q, out, lse, rows=20)
 
 
+def test_attention_stays_within_the_hosts_bounds(dev):
+    """Arrays on the device that pass the bounds of the host: of a longer q_len
+    the first max_q_len rows are computed, at the positions that the arrays say;
+    a longer kv_len counts as max_kv_len; other rows keep what they hold."""
+    for name, max_q in (("mixed", 20), ("drafts", 2), ("prompts", 64)):
+        n, lens, hq, hkv, d, page = ATTENTION[name]
+        c = R.Case(n, lens, hq, hkv, d, page, F16, seed=12, pad=2)
+        q, kp, vp = c.normal(c.T, hq, d), c.normal(c.total, hkv, page, d), c.normal(c.total, hkv, d, page)
+        want, _ = _attention(dev, c, kp, vp, q)
+        kv, b = ops.PagedKVCache(dev, kp, vp), c.batch(ops, max_q=max_q)
+        out = torch.full((c.T, hq, d), 7.0, dtype=F16, device="cuda")
+        ws = torch.full((max(16, ops.paged_attention_workspace_bytes(kv, b, hq)),), 255, dtype=torch.uint8, device="cuda")
+        ops.dispatch_paged_attention(dev, kv, b, q, out, ws)
+        dev.sync()
+        for s, (m, st) in enumerate(zip(n, c.starts)):
+            _near(out[st:st + min(m, max_q)], want[st:st + min(m, max_q)])
+            assert (out[st + min(m, max_q):st + m] == 7.0).all()
+        assert (out[c.rows:] == 7.0).all()
+        short = max(1, max(lens) // 2)
+        b = c.batch(ops, max_kv=short)
+        d2 = R.Case(n, [min(l, short) for l in lens], hq, hkv, d, page, F16, seed=12, pad=2)
+        d2.table, d2.total = c.table, c.total
+        out = torch.full((c.T, hq, d), 7.0, dtype=F16, device="cuda")
+        lse = torch.full((c.T, hq), 7.0, device="cuda")
+        ops.dispatch_paged_attention(dev, kv, b, q, out, ws.new_full((max(16, ops.paged_attention_workspace_bytes(kv, b, hq)),), 255), lse=lse)
+        dev.sync()
+        _check_attention(d2, kp, vp, q, out, lse, rows=16)
+
+
+def _near(a, b):
+    """Two calls that split the same keys differently: their float32 sums differ by
+    the order, and by what weights and stores then round to (half a step each way)."""
+    assert ((a.double() - b.double()).abs() <= 4 * 2.0 ** -11 * b.double().abs().amax(-1, keepdim=True) + 1e-6).all()
+
+
+@pytest.mark.parametrize("page", [256, 1024])
+def test_attention_over_large_pages_into_strided_rows(dev, page):
+    c = R.Case([1, 70, 2], [2100, 500, 1030], 6, 2, 64, page, BF16, seed=13)
+    q, kp, vp = c.normal(c.T, 6, 64), c.normal(c.total, 2, page, 64), c.normal(c.total, 2, 64, page)
+    kv, b = ops.PagedKVCache(dev, kp, vp), c.batch(ops)
+    rows = torch.full((c.T, 6 * 64 + 40), 7.0, dtype=BF16, device="cuda")
+    out = rows[:, 8:8 + 6 * 64].unflatten(1, (6, 64))
+    lse = torch.zeros(c.T, 6, device="cuda")
+    ws = torch.full((max(16, ops.paged_attention_workspace_bytes(kv, b, 6)),), 255, dtype=torch.uint8, device="cuda")
+    ops.dispatch_paged_attention(dev, kv, b, q, out, ws, lse=lse)
+    dev.sync()
+    _check_attention(c, kp, vp, q, out, lse, rows=16)
+    assert (rows[:, :8] == 7.0).all() and (rows[:, 8 + 6 * 64:] == 7.0).all()
+
+
+def test_many_sequences(dev):
+    """More sequences than a wave looks through at once, some of them empty."""
+    r = random.Random(3)
+    n = [r.choice([0, 0, 1, 1, 2, 17]) for _ in range(300)]
+    lens = [m + r.randint(0, 60) for m in n]
+    c = R.Case(n, lens, 4, 2, 64, 16, F16, seed=14, pad=5)
+    q, kp, vp = c.normal(c.T, 4, 64), c.normal(c.total, 2, 16, 64), c.normal(c.total, 2, 64, 16)
+    out, lse = _attention(dev, c, kp, vp, q)
+    _check_attention(c, kp, vp, q, out, lse, rows=40)
+    k, v = c.normal(c.T, 2, 64), c.normal(c.T, 2, 64)
+    kv = ops.PagedKVCache(dev, kp.clone(), vp.clone())
+    q_out = torch.zeros_like(q)
+    ops.dispatch_paged_append(dev, kv, c.batch(ops), q, k, v, q_out, rotary_dim=0)
+    dev.sync()
+    ks, vs = kp.clone(), vp.clone()
+    for row, s, pos in c.rows_of():
+        p = int(c.table[s, pos // 16])
+        ks[p, :, pos % 16], vs[p, :, :, pos % 16] = k[row], v[row]
+    assert same(kv.k_pages, ks) and same(kv.v_pages, vs)
+    assert same(q_out[:c.rows], q[:c.rows]) and not q_out[c.rows:].any()
+
+
 def test_far_pages(dev):
     """Pages whose byte offsets pass 32 bits, in K and in V."""
     c = R.Case([1, 90], [900, 300], 8, 8, 128, 16, F16, seed=2, first_page=140_000)

@@ -114,7 +114,8 @@ def test_append_in_place_needs_one_stride(h):
 @pytest.mark.parametrize("p", [
     dict(num_query_heads=3), dict(num_query_heads=0), dict(num_query_heads=2048), dict(q_stride=256),
     dict(out_stride=513), dict(scale=-1.), dict(scale=float("inf")), dict(softcap=-1.),
-    dict(softcap=float("nan")), dict(slopes=A + 1), dict(prefix_lens=A + 2)])
+    dict(softcap=float("nan")), dict(softcap=1e-30), dict(softcap=1e7), dict(scale=1e-38), dict(scale=2e30),
+    dict(scale=float("nan")), dict(slopes=A + 1), dict(prefix_lens=A + 2)])
 def test_attention_parameters_are_checked(h, p):
     assert _attn(h, **p)[0] == L.EINVAL
 
@@ -129,6 +130,7 @@ def test_attention_buffers_are_checked(h, at):
     (dict(top_n=65, vocab=200, row_stride=200), {}, L.EINVAL), (dict(top_n=101), {}, L.EINVAL),
     (dict(vocab=4, top_n=5), {}, L.EINVAL), (dict(dtype=3), {}, L.EINVAL), (dict(temperature=0.), {}, L.EINVAL),
     (dict(temperature=float("nan")), {}, L.EINVAL), (dict(temperature=float("inf")), {}, L.EINVAL),
+    (dict(temperature=1e-38), {}, L.EINVAL), (dict(temperature=-1.), {}, L.EINVAL), (dict(rows=1 << 24), {}, L.EINVAL),
     (dict(vocab=(1 << 28) + 1, row_stride=1 << 29), {}, L.EINVAL), ({}, dict(x=A + 2), L.EINVAL),
     (dict(dtype=L.F16), dict(x=A + 2), L.OK), ({}, dict(lp=None), L.EINVAL), ({}, dict(tokens=None), L.EINVAL),
     (dict(top_n=3), dict(ids=None, top=None), L.EINVAL), (dict(top_n=3), dict(ids=None), L.OK)])
@@ -149,6 +151,14 @@ def test_null_context_and_workspace_size_need_no_gpu():
                                            None) == L.EINVAL
     assert lib.nnz_paged_attention_workspace_bytes(None, None, 4) == 0
     assert lib.nnz_paged_attention_workspace_bytes(C.byref(kv(head_dim=96)), C.byref(batch()), 4) == 0
+
+
+def test_struct_layouts(h):
+    """The same numbers are asserted of the C structs where paged_host.cc is compiled."""
+    for t, size, field, at in ((L.PagedKV, 40, "dtype", 32), (L.PagedBatchDesc, 48, "max_kv_len", 40),
+                               (L.PagedAppendParams, 64, "eps", 56), (L.PagedAttnParams, 40, "softcap", 36),
+                               (L.LogprobsDims, 32, "temperature", 24)):
+        assert C.sizeof(t) == size and getattr(t, field).offset == at
 
 
 # ------------------------------------------------------------ index arithmetic
@@ -272,7 +282,7 @@ def test_rows_of_another_shape_or_type_are_refused():
         with pytest.raises(NnzError):
             ops.dispatch_paged_append(CPU, c, b, **a)
     for bad in (dict(q=q[:, :, :32]), dict(out=q[:3]), dict(lse=torch.zeros(4, 6)), dict(slopes=torch.zeros(2)),
-                dict(prefix_lens=torch.zeros(2)), dict(prefix_lens=torch.zeros(3, dtype=torch.int32))):
+                dict(window=-1), dict(prefix_lens=torch.zeros(2)), dict(prefix_lens=torch.zeros(3, dtype=torch.int32))):
         a = {**dict(q=q, out=q.clone(), workspace=None), **bad}
         with pytest.raises(NnzError):
             ops.dispatch_paged_attention(CPU, c, b, **a)
