@@ -574,7 +574,8 @@ int nnz_dispatch_paged_append(nnz_ctx *ctx, const nnz_paged_kv *kv, const nnz_pa
  * are all -inf, gives zeros and lse -inf.  What masked positions hold,
  * infinities and NaN included, has no influence.
  * Scores, softmax and sums are f32; the weights are rounded to the cache's
- * type for the product with V.
+ * type for the product with V.  Biases are added in units of q.k:
+ * slopes[h] * |p - j| / scale has to be finite in f32.
  * workspace: nnz_paged_attention_workspace_bytes(kv, batch, num_query_heads)
  * bytes (0 = none needed), 16-byte aligned; its contents do not matter before
  * or after.  Calls that overlap, captured ones among them, need one each. */

@@ -55,6 +55,7 @@ struct AttnArgs {
     uint64_t q_stride, o_stride;
     uint32_t hq, G, window;
     float scale;          // of the scores, times log2 e
+    float unbias;         // 1 / scale before that: a bias in units of products
     float cap_in, cap;    // softcap: cap * tanh(x) with 2 log2(e) x = cap_in * (q . k); cap times log2 e
     // Sequences of at most `few` rows (0: none) are few_part's: keys in chunks of
     // few_steps steps, at most few_splits of them, a block each, few_blocks in all.
@@ -110,24 +111,25 @@ __device__ __forceinline__ float odd_value(uint16_t v, bool seen) {
     return seen && !(fabsf(f) < INFINITY) ? f : 0.f;
 }
 
-// How a product becomes a score: plain ones stay products and are scaled in the
-// exponent, the others are put into log2 units first.
-enum { PLAIN, BIASED, CAPPED };   // CAPPED: biased too where there are slopes
+// How a product becomes a score.  Without a softcap scores stay in units of
+// products, a bias too, and are scaled in the exponent; capped ones are in log2 units.
+enum { PLAIN, BIASED, CAPPED, CAPPED_BIASED };
+constexpr bool biased(int sc) { return sc & 1; }
+constexpr bool capped(int sc) { return sc & 2; }
 template <int SC>
 __device__ __forceinline__ float score_of(const AttnArgs &a, float s, float slope, int32_t distance) {
-    if constexpr (SC == PLAIN) return s;
-    float t = a.scale * s;
-    if constexpr (SC == CAPPED)   // tanh(x) = 1 - 2 / (e^2x + 1)
-        t = a.cap * fmaf(-2.f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(a.cap_in * s) + 1.f), 1.f);
-    return fmaf(-slope, fabsf((float)distance), t);
+    if constexpr (capped(SC))   // tanh(x) = 1 - 2 / (e^2x + 1)
+        s = a.cap * fmaf(-2.f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(a.cap_in * s) + 1.f), 1.f);
+    if constexpr (biased(SC)) s = fmaf(-slope, fabsf((float)distance), s);
+    return s;
 }
 
 // ---------------------------------------------------------------- few rows
 // A step is 32 keys of a wave: K as two A operands of 16 keys (row m of operand
 // i is key 8 (m >> 2) + 4 i + (m & 3), so lane group g's accumulators hold keys
-// 8 g .. 8 g + 7), V^T as D/16 A operands.  The next step's loads are issued
-// before the current one is computed.  Block = W waves that take the steps of
-// a chunk in turn.
+// 8 g .. 8 g + 7), V^T as D/16 A operands.  With AHEAD the next step's loads are
+// issued before the current one is computed.  Block = W waves that take the steps
+// of a chunk in turn.
 template <int D, bool BF>
 struct FewStep {
     v4u k[2][D / 32], v[D / 16];
@@ -140,7 +142,7 @@ struct FewShared {
     float m[W][16], l[W][16];
 };
 
-template <int D, bool BF, int SC, int W>
+template <int D, bool BF, int SC, int W, bool AHEAD>
 __device__ __forceinline__ void few_part(const AttnArgs &a, uint32_t block, FewShared<D, W> &sh) {
     constexpr int NKS = D / 32, NDT = D / 16;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -160,7 +162,7 @@ __device__ __forceinline__ void few_part(const AttnArgs &a, uint32_t block, FewS
     const uint32_t r = paged_min((uint32_t)c, R - 1), tok = r / a.G, head = kvh * a.G + r % a.G;
     const int32_t pos = sq.first + (int32_t)tok;
     const PagedSpan sp = paged_span(pos, sq.len, prefix, a.window);
-    const float slope = SC != PLAIN && a.slopes ? a.slopes[head] * LOG2E : 0.f;
+    const float slope = biased(SC) ? a.slopes[head] * (capped(SC) ? LOG2E : a.unbias) : 0.f;
     v4u qf[NKS];
     {
         const uint16_t *qp = a.q + (sq.row0 + tok) * a.q_stride + head * D;
@@ -194,7 +196,7 @@ __device__ __forceinline__ void few_part(const AttnArgs &a, uint32_t block, FewS
     float4v o[NDT];
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt) o[dt] = (float4v){0.f, 0.f, 0.f, 0.f};
-    const float cs = SC == PLAIN ? a.scale : 1.f, ahead = 8.f / cs;
+    const float cs = capped(SC) ? 1.f : a.scale, ahead = 8.f / cs;
     float m = -INFINITY, nm = 0.f, l = 0.f;   // reference score, minus it in log2 units, sum of this lane's weights
     uint32_t odd = 0;
     auto in_part = [&](uint32_t k0, uint32_t bad) { return k0 < sp1.lo || k0 + 32 > sp0.hi || bad; };   // wave-uniform
@@ -251,7 +253,13 @@ __device__ __forceinline__ void few_part(const AttnArgs &a, uint32_t block, FewS
     };
 
     uint32_t st = z * a.few_steps + (uint32_t)w;
-    if (st < st1) {   // wave-uniform, all of it
+    if constexpr (!AHEAD) {
+        for (; st < st1; st += W) {   // wave-uniform
+            FewStep<D, BF> f;
+            load(f, st);
+            compute(f, st);
+        }
+    } else if (st < st1) {   // wave-uniform, all of it
         FewStep<D, BF> f0, f1;
         load(f0, st);
         for (;;) {
@@ -277,10 +285,12 @@ __device__ __forceinline__ void few_part(const AttnArgs &a, uint32_t block, FewS
                 const uint16_t *vp = vh + (uint64_t)page * page_len + (key & pmask);
                 const bool seen = key >= sp.lo && key < sp.hi;
 #pragma unroll
-                for (int dt = 0; dt < NDT; ++dt)
+                for (int dt = 0; dt < NDT; ++dt) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        o[dt][e] += odd_value<BF>(vp[(size_t)(16 * dt + 4 * g + e) << a.b.shift], seen);
+                        o[dt][e] += odd_value<BF>(vp[(16 * dt + 4 * g + e) << a.b.shift], seen);
+                    __builtin_amdgcn_sched_barrier(0);   // all loads at once would take registers
+                }
             }
         }
     }
@@ -422,19 +432,18 @@ __device__ __forceinline__ void chunk_part(const AttnArgs &a, uint32_t block, Ch
     const PagedSpan first = span_of(paged_min(w0, rt.R - 1)), last = span_of(wl), sp = span_of(r);
     const uint32_t tok = r / a.G, head = kvh * a.G + r % a.G;
     const int32_t pos = rt.sq.first + (int32_t)tok;
-    const float slope = SC != PLAIN && a.slopes ? a.slopes[head] * LOG2E : 0.f;
-    const int32_t first_pos = rt.sq.first + (int32_t)(paged_min(w0, rt.R - 1) / a.G);
+    const float slope = biased(SC) ? a.slopes[head] * (capped(SC) ? LOG2E : a.unbias) : 0.f;
 
     // Wave w stages group w of a tile's four groups of 16 keys, K and V alike:
     // one page.  Piece i of a lane: 16 bytes of K row 64 i / PIECES + lane / PIECES,
     // of V^T row 32 i + lane / 2.
     constexpr uint32_t RPW = 64 / PIECES;   // K rows of the wave's piece
-    uint32_t koff[LOADS], voff[LOADS];
+    uint32_t koff[LOADS];
+    const uint32_t voff = (((uint32_t)lane / 2) << a.b.shift) * 2u + ((uint32_t)lane & 1) * 16u;
 #pragma unroll
     for (uint32_t i = 0; i < LOADS; ++i) {
         const uint32_t row = i * RPW + (uint32_t)lane / PIECES;
         koff[i] = (row * D + 8 * (((uint32_t)lane % PIECES) ^ (row & (PIECES - 1)))) * 2u;
-        voff[i] = ((32 * i + (uint32_t)lane / 2) << a.b.shift) * 2u + ((uint32_t)lane & 1) * 16u;
     }
     // elements of a page; this head's part of page 0
     const uint32_t pmask = (1u << a.b.shift) - 1, page_len = (hkv * D) << a.b.shift;
@@ -462,7 +471,7 @@ __device__ __forceinline__ void chunk_part(const AttnArgs &a, uint32_t block, Ch
 #pragma unroll
         for (uint32_t i = 0; i < LOADS; ++i) {
             load_to_lds(kp, koff[i], lds_k + buf + 1024 * i);
-            load_to_lds(vp, voff[i], lds_v + buf + 1024 * i);
+            load_to_lds(vp + ((32 * i) << a.b.shift), voff, lds_v + buf + 1024 * i);
         }
     };
     auto bad_of = [&](const Pages &p, uint32_t t) __attribute__((always_inline)) {
@@ -493,9 +502,9 @@ __device__ __forceinline__ void chunk_part(const AttnArgs &a, uint32_t block, Ch
     for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[dt][e] = 0.f;
-    const float cs = SC == PLAIN ? a.scale : 1.f, ahead = 8.f / cs;
+    const float cs = capped(SC) ? 1.f : a.scale, ahead = 8.f / cs;
     float m = -INFINITY, nm = 0.f, l = 0.f;
-    uint32_t odd = 0;
+    bool odd = false;   // wave-uniform
     // tiles that some rows of the wave, of the block, see only in part
     auto in_part = [&](uint32_t k0, uint32_t gone) { return k0 < last.lo || k0 + KT > first.hi || gone; };
     const uint32_t lo_most = span_of(paged_min(rt.r0 + TILE_ROWS, rt.R) - 1).lo, hi_least = span_of(rt.r0).hi;
@@ -523,7 +532,7 @@ __device__ __forceinline__ void chunk_part(const AttnArgs &a, uint32_t block, Ch
                 uint32_t met = 0;
                 const v4u v = finite_part<BF>(*at, met);
                 if (met) *at = v;
-                odd |= met;
+                odd |= __builtin_amdgcn_ballot_w64(met != 0) != 0;
             }
             __builtin_amdgcn_s_waitcnt(7 << 4);
         }
@@ -538,6 +547,9 @@ __device__ __forceinline__ void chunk_part(const AttnArgs &a, uint32_t block, Ch
             barrier();
             continue;
         }
+        // computed anew in every turn where registers are short: the asm hides that they need not be
+        uint32_t krow = krm * D + 8 * (hh ^ (krm & (PIECES - 1)));
+        if constexpr (D == 64) asm volatile("" : "+v"(krow));
         const uint16_t *const Kt = sh.k[group][i & 1], *const Vt = sh.v[group][i & 1];
         // scores of both halves of the tile; the operands of a half are all read
         // before its products, the second half's during the first one's
@@ -545,10 +557,8 @@ __device__ __forceinline__ void chunk_part(const AttnArgs &a, uint32_t block, Ch
         v4u kf[2][NKS];
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) {
-            const int row = 32 * kt + krm;
 #pragma unroll
-            for (int ks = 0; ks < NKS; ++ks)
-                kf[kt][ks] = *(const v4u *)(Kt + row * D + 8 * ((2 * ks + hh) ^ (row & (PIECES - 1))));
+            for (int ks = 0; ks < NKS; ++ks) kf[kt][ks] = *(const v4u *)(Kt + 32 * kt * D + (krow ^ 16 * ks));
             __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
@@ -571,24 +581,26 @@ __device__ __forceinline__ void chunk_part(const AttnArgs &a, uint32_t block, Ch
         // over 8192 184.9 and 179.1 us, 1500 over 3000 76.2 and 72.6; at 64, 102 and
         // 103 (capped), 51.3 and 54.0 (five prompts, biased)
         if constexpr (D == 128) __builtin_amdgcn_s_setprio(1);
-        const uint32_t key = k0 + 8 * hh;   // register e of half kt: key + 32 kt + 16 (e >> 3) + (e & 7)
-        if constexpr (SC == CAPPED) {
+        uint32_t key = k0 + 8 * hh;   // register e of half kt: key + 32 kt + 16 (e >> 3) + (e & 7)
+        int32_t rel = pos - (int32_t)key;
+        if constexpr (D == 64) asm volatile("" : "+v"(key), "+v"(rel));
+        auto few_at_once = [](int e) __attribute__((always_inline)) {   // chains in flight take registers
+            if (D == 64 && e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+        };
+        if constexpr (capped(SC)) {
             const float cap2 = -2.f * a.cap;
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
+            for (int e = 0; e < 32; ++e) {
                 sc[e >> 4][e & 15] = fmaf(cap2, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(a.cap_in * sc[e >> 4][e & 15]) + 1.f), a.cap);
+                few_at_once(e);
+            }
         }
-        if (SC == BIASED || (SC == CAPPED && a.slopes)) {   // uniform
-            const float by = SC == BIASED ? a.scale : 1.f;
-            if ((int32_t)(k0 + KT) <= first_pos + 1) {   // wave-uniform: no key after any row
-                const float near = -slope * (float)(pos - (int32_t)key);
+        if constexpr (biased(SC)) {
+            const float d = (float)rel;   // distances are exact up to 2^24, and as good as the scores beyond
 #pragma unroll
-                for (int e = 0; e < 32; ++e)
-                    sc[e >> 4][e & 15] = fmaf(sc[e >> 4][e & 15], by, fmaf(slope, (float)(16 * (e >> 3) + (e & 7)), near));
-            } else {
-#pragma unroll
-                for (int e = 0; e < 32; ++e)
-                    sc[e >> 4][e & 15] = fmaf(-slope, fabsf((float)(pos - (int32_t)(key + 16 * (e >> 3) + (e & 7)))), by * sc[e >> 4][e & 15]);
+            for (int e = 0; e < 32; ++e) {
+                sc[e >> 4][e & 15] = fmaf(-slope, fabsf(d - (float)(16 * (e >> 3) + (e & 7))), sc[e >> 4][e & 15]);
+                few_at_once(e);
             }
         }
         const bool masked = in_part(k0, bad);
@@ -598,6 +610,7 @@ __device__ __forceinline__ void chunk_part(const AttnArgs &a, uint32_t block, Ch
                 const uint32_t j = key + 16 * (e >> 3) + (e & 7);
                 const bool on = j >= sp.lo && j < sp.hi && !(bad >> (e >> 3) & 1);
                 sc[e >> 4][e & 15] = on ? sc[e >> 4][e & 15] : -INFINITY;
+                few_at_once(e);
             }
         }
         float mx = sc[0][0];
@@ -653,8 +666,7 @@ __device__ __forceinline__ void chunk_part(const AttnArgs &a, uint32_t block, Ch
     const float2 lp = swap32(l, l);
     l = lp.x + lp.y;
     float M = m == -INFINITY ? -INFINITY : -nm;
-    const bool met = __builtin_amdgcn_ballot_w64(odd != 0) != 0;
-    if (lane == 0) sh.odd[group][wave] = met;
+    if (lane == 0) sh.odd[group][wave] = odd;
     __syncthreads();
     if (__builtin_expect(sh.odd[group][0] | sh.odd[group][1] | sh.odd[group][2] | sh.odd[group][3], 0)) {   // group-uniform
         for (uint32_t t = ta; t < t1; t += 2) {
@@ -666,78 +678,95 @@ __device__ __forceinline__ void chunk_part(const AttnArgs &a, uint32_t block, Ch
                 const uint16_t *vp = vh + (uint64_t)page * page_len + (key & pmask);
                 const bool seen = key >= sp.lo && key < sp.hi;
 #pragma unroll
-                for (int dt = 0; dt < NDT; ++dt)
+                for (int dt = 0; dt < NDT; ++dt) {
 #pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        o[dt][e] += odd_value<BF>(vp[(size_t)(32 * dt + 8 * (e >> 2) + 4 * hh + (e & 3)) << a.b.shift], seen);
+                    for (int e = 0; e < 16; ++e) {
+                        o[dt][e] += odd_value<BF>(vp[(32 * dt + 8 * (e >> 2) + 4 * hh + (e & 3)) << a.b.shift], seen);
+                        if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
             }
         }
     }
+    // where the lane's results go, computed here: kept over the loop that costs registers
+    uint32_t none = 0, G = a.G;
+    asm volatile("" : "+s"(none), "+s"(G));
+    const uint32_t ln = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, none)), lh = ln >> 5, row = w0 + (ln & 31);
     float (&join)[D / 2 + 2][64] = sh.join[wave];
     if (group) {
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) join[16 * dt + e][lane] = o[dt][e];
-        join[D / 2][lane] = M;
-        join[D / 2 + 1][lane] = l;
+            for (int e = 0; e < 16; ++e) join[16 * dt + e][ln] = o[dt][e];
+        join[D / 2][ln] = M;
+        join[D / 2 + 1][ln] = l;
     }
     __syncthreads();
-    if (group || !any || w0 + (uint32_t)c >= rt.R) return;
+    if (group || !any || row >= rt.R) return;
     {
-        const float M2 = join[D / 2][lane], to = fmaxf(M, M2);
+        const float M2 = join[D / 2][ln], to = fmaxf(M, M2);
         const float f = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - to);
         const float f2 = M2 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M2 - to);
-        l = l * f + join[D / 2 + 1][lane] * f2;
+        l = l * f + join[D / 2 + 1][ln] * f2;
         M = to;
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) o[dt][e] = o[dt][e] * f + join[16 * dt + e][lane] * f2;
+            for (int e = 0; e < 16; ++e) o[dt][e] = o[dt][e] * f + join[16 * dt + e][ln] * f2;
     }
     if (rt.nz > 1) {
-        const size_t part = (((size_t)u * hkv + kvh) * a.chunk_splits + z) * TILE_ROWS + (w0 - rt.r0) + (uint32_t)c;
+        const size_t part = (((size_t)u * hkv + kvh) * a.chunk_splits + z) * TILE_ROWS + (row - rt.r0);
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                *(float4v *)(a.chunk_o + part * D + 32 * dt + 8 * j + 4 * hh) =
+                *(float4v *)(a.chunk_o + part * D + 32 * dt + 8 * j + 4 * lh) =
                     (float4v){o[dt][4 * j], o[dt][4 * j + 1], o[dt][4 * j + 2], o[dt][4 * j + 3]};
-        if (hh == 0) {
+        if (lh == 0) {
             a.chunk_ml[2 * part] = M;
             a.chunk_ml[2 * part + 1] = l;
         }
         return;
     }
+    const uint32_t of = row / G, hd = kvh * G + row % G;   // token, head
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    uint16_t *const op = a.out + (rt.sq.row0 + tok) * a.o_stride + head * D;
+    uint16_t *const op = a.out + (rt.sq.row0 + of) * a.o_stride + hd * D;
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            *(uint2 *)(op + 32 * dt + 8 * j + 4 * hh) =
+            *(uint2 *)(op + 32 * dt + 8 * j + 4 * lh) =
                 make_uint2(pack2<BF>(o[dt][4 * j] * inv, o[dt][4 * j + 1] * inv),
                            pack2<BF>(o[dt][4 * j + 2] * inv, o[dt][4 * j + 3] * inv));
-    if (a.lse && hh == 0)
-        a.lse[(size_t)(rt.sq.row0 + tok) * a.hq + head] = l == 0.f ? -INFINITY : (M + __builtin_amdgcn_logf(l)) * LN2;
+    if (a.lse && lh == 0)
+        a.lse[(size_t)(rt.sq.row0 + of) * a.hq + hd] = l == 0.f ? -INFINITY : (M + __builtin_amdgcn_logf(l)) * LN2;
 }
 
-// One launch for a batch: few_part's blocks first (they wait for memory while
-// the chunks' compute).
+// One launch for a batch, chunk_part's blocks first: they take longest, and
+// few_part's then fill the CUs beside them.  Measured with few_part's first and
+// last: 18 single tokens and 6 chunks in a window of 512 (head_dim 64, capped)
+// 31.9 and 24.5 us, at head_dim 128 41.3 and 38.8, 24 sequences without a window
+// 90.3 and 93.1.
+// At head_dim 64 chunk_part keeps to 128 registers, so that a CU holds two of its
+// blocks; few_part beside it then has no room to load a step ahead, and need not,
+// with four waves a SIMD (24 sequences, 1 and 2 blocks a CU: 40.8 and 33.8 us).
 enum { FEW_4, FEW_8, CHUNK, BOTH };   // few_part by 4 or 8 waves, chunk_part, both
 constexpr int threads_of(int kind) { return kind == FEW_4 ? 256 : 512; }
+constexpr int waves_of(int head_dim, int kind) { return head_dim == 64 && (kind == CHUNK || kind == BOTH) ? 4 : 2; }
 template <int D, bool BF, int SC, int KIND>
-__global__ __launch_bounds__(threads_of(KIND)) __attribute__((amdgpu_waves_per_eu(2))) void attn_kernel(AttnArgs a) {
+__global__ __launch_bounds__(threads_of(KIND)) __attribute__((amdgpu_waves_per_eu(waves_of(D, KIND)))) void attn_kernel(AttnArgs a) {
     constexpr int W = threads_of(KIND) / 64;
+    constexpr bool AHEAD = waves_of(D, KIND) == 2;
     __shared__ __align__(16) union {
         char none;
         typename std::conditional<KIND != CHUNK, FewShared<D, W>, char>::type few;
         typename std::conditional<KIND == CHUNK || KIND == BOTH, ChunkShared<D>, char>::type chunk;
     } sh;
+    const uint32_t chunk_blocks = gridDim.x - a.few_blocks;
     if constexpr (KIND == CHUNK) chunk_part<D, BF, SC>(a, blockIdx.x, sh.chunk);
-    else if constexpr (KIND != BOTH) few_part<D, BF, SC, W>(a, blockIdx.x, sh.few);
-    else if (blockIdx.x < a.few_blocks) few_part<D, BF, SC, W>(a, blockIdx.x, sh.few);
-    else chunk_part<D, BF, SC>(a, blockIdx.x - a.few_blocks, sh.chunk);
+    else if constexpr (KIND != BOTH) few_part<D, BF, SC, W, AHEAD>(a, blockIdx.x, sh.few);
+    else if (blockIdx.x < chunk_blocks) chunk_part<D, BF, SC>(a, blockIdx.x, sh.chunk);
+    else few_part<D, BF, SC, W, AHEAD>(a, blockIdx.x - chunk_blocks, sh.few);
 }
 
 // ------------------------------------------------------------- parts joined
@@ -926,7 +955,8 @@ void start(hipStream_t stream, const Plan &p, AttnArgs a, float *ws) {
 
 template <int D, bool BF>
 void start_scores(hipStream_t stream, const Plan &p, const AttnArgs &a, float *ws) {
-    if (a.cap > 0.f) start<D, BF, CAPPED>(stream, p, a, ws);
+    if (a.cap > 0.f && a.slopes) start<D, BF, CAPPED_BIASED>(stream, p, a, ws);
+    else if (a.cap > 0.f) start<D, BF, CAPPED>(stream, p, a, ws);
     else if (a.slopes) start<D, BF, BIASED>(stream, p, a, ws);
     else start<D, BF, PLAIN>(stream, p, a, ws);
 }
@@ -968,6 +998,7 @@ extern "C" int nnz_dispatch_paged_attention(nnz_ctx *ctx, const nnz_paged_kv *kv
     a.window = p->window;
     const float scale = p->scale > 0.f ? p->scale : 1.f / sqrtf((float)kv->head_dim);
     a.scale = scale * LOG2E;
+    a.unbias = 1.f / scale;
     a.cap = p->softcap * LOG2E;
     a.cap_in = p->softcap > 0.f ? 2.f * LOG2E * scale / p->softcap : 0.f;
     const bool bf = kv->dtype == NNZ_BF16;
