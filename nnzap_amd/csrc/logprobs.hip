@@ -548,6 +548,7 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(LpArgs a) {
 }
 
 // Blocks for about four per CU, each with a group of values per lane at least.
+// (512, 1024 and 2048 blocks: 333 x 50257 bf16 34.8, 25.0 and 31.0 us.)
 // At most 96: the join's keys (64 each) stay within 48 KB of LDS.
 uint32_t pieces_of(uint32_t rows, uint32_t vocab) {
     const uint32_t want = std::max(1u, 1024u / rows), most = std::max(1u, vocab / (WAVES * 64 * GROUP));

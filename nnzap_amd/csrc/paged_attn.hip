@@ -19,6 +19,13 @@
 //               and over blocks where there are few rows.
 // join_kernel joins what blocks computed of one row.
 //
+// Measured (kernels' time): one token over 131072 (32 + 8 heads of 128, bf16, 537
+// MB) 95 + 8 us, 5.6 TB/s; 64 chats of up to 8191 (1.17 GB) 238 + 5, 4.9 TB/s; 2048
+// tokens over 8192 (16 + 8 heads of 128, 155 GFLOP) 171 us, 0.9 PFLOP/s: there 256
+// KB of LDS reads a turn take 3000 of a CU's 4400 cycles, vector instructions 2600,
+// the matrix cores 2048; 64 rows a wave would halve the reads, but leave one wave
+// a SIMD.
+//
 // The softmax is the online one in base 2: sums are kept relative to a
 // reference M per row, which follows the row's maximum only when that runs
 // ahead by more than 2^8 (weights up to 2^8 cost no precision: f16 and bf16
@@ -773,6 +780,9 @@ __global__ __launch_bounds__(threads_of(KIND)) __attribute__((amdgpu_waves_per_e
 // A row takes D/4 threads (four dims each) times 1, 2, 4 or 8 sets that share
 // its parts out; a block holds as many rows as fit.  few_part's rows first, by
 // (sequence, KV head, row), then chunk_part's, by (row tile, KV head, row).
+// Bound by its loads' latency: with one set everywhere one token over 131072 keys
+// takes 130 us for 104, over 16000 23.5 for 19.3; with eight 12 sequences of chunks
+// and single tokens 260 for 236.
 constexpr uint32_t MOST_SPLITS = 256;
 struct JoinArgs {
     uint64_t few_rows;            // rows of few_part's, rounded up to whole blocks
@@ -882,6 +892,18 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a, JoinArgs j) {
 
 // ------------------------------------------------------------------- launch
 // Which parts run and how keys are split, from the host's bounds alone.
+// few_part: about 1024 blocks (one token over 131072: 512, 1024 and 2048 blocks
+// 101, 104 and 111 us; 64 chats 251, 243 and 239), of 16 steps at least (8, 16 and
+// 32: 513 keys 13.7, 10.0 and 10.6 us, four tokens over 2000 14.7, 16.0 and 26,
+// 32 over 500-1500 at head_dim 64 19.6, 17.1 and 15.6); 256 beside chunks (more
+// change nothing).
+// chunk_part: as many blocks as the CUs hold, 256 at head_dim 128 and 512 at 64
+// (512 tokens over 25000, 256 and 512 blocks: 132 and 146 us, 85 and 76); 512 for
+// several sequences, whose lengths differ and whose row tiles are bounded from
+// above only (12 of up to 30300 keys, head_dim 128, 311 and 235 us, three prompts
+// 75 and 64; two prompts of one length lose, 54 and 61); four tiles of keys at
+// least (2 and 4: 300 tokens alone 17.5 and 13.4 us; 8 and 4: 64 over 2000 21.7 and
+// 19.0).
 struct Plan {
     uint32_t few_rows = 0, few_splits = 0, few_steps = 0;          // 0 splits: not launched
     uint32_t units = 0, chunk_splits = 0, chunk_tiles = 0;
@@ -909,7 +931,8 @@ Plan plan_of(const nnz_paged_kv &kv, const nnz_paged_batch &b, uint32_t hq) {
         const uint64_t by_seqs = (uint64_t)b.num_seqs * ((most + TILE_ROWS - 1) / TILE_ROWS);
         p.units = (uint32_t)std::min(by_rows, by_seqs);
         const uint32_t tiles = (b.max_kv_len + KT - 1) / KT;
-        const uint32_t want = (uint32_t)std::max<uint64_t>(1, 256 / ((uint64_t)p.units * hkv)), most_splits = std::max(1u, tiles / 4);
+        const uint32_t blocks = kv.head_dim == 64 || b.num_seqs > 1 ? 512 : 256;
+        const uint32_t want = (uint32_t)std::max<uint64_t>(1, blocks / ((uint64_t)p.units * hkv)), most_splits = std::max(1u, tiles / 4);
         const uint32_t splits = std::min({want, most_splits, MOST_SPLITS});
         p.chunk_tiles = (tiles + splits - 1) / splits;
         p.chunk_splits = (tiles + p.chunk_tiles - 1) / p.chunk_tiles;
@@ -939,6 +962,9 @@ void start(hipStream_t stream, const Plan &p, AttnArgs a, float *ws) {
     a.chunk_o = a.few_ml + p.few_parts * 2;
     a.chunk_ml = a.chunk_o + p.chunk_parts * D;
     const uint32_t chunk_blocks = p.units * hkv * p.chunk_splits;
+    // 8 waves a block where blocks are fewer than CUs (4 and 8: one token over 4000
+    // 16.3 and 15.3 us), 4 beyond, two blocks a CU (8 and 4: 131072 107 and 104, 64
+    // chats 245 and 242)
     if (!chunk_blocks && a.few_blocks > 256) attn_kernel<D, BF, SC, FEW_4><<<a.few_blocks, 256, 0, stream>>>(a);
     else if (!chunk_blocks) attn_kernel<D, BF, SC, FEW_8><<<a.few_blocks, 512, 0, stream>>>(a);
     else if (!a.few_blocks) attn_kernel<D, BF, SC, CHUNK><<<chunk_blocks, 512, 0, stream>>>(a);
