@@ -28,7 +28,7 @@ typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 // computed once into LDS.  V goes to its transposed page two dims a lane, all
 // positions of the group in registers: whole groups are two 16-byte stores.
 // q and k leave past the caches: 8192 tokens of 32 + 8 heads 60 -> 55 us (201 MB,
-// 3.7 TB/s), 4093 tokens of seven prompts 31 -> 26 us; V's 16-byte pieces not,
+// 3.7 TB/s), 4093 tokens of seven prompts 30 -> 25 us; V's 16-byte pieces not,
 // they meet in the L2 (past it: 70 us).
 template <int D, bool BF>
 __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
