@@ -910,15 +910,21 @@ struct Plan {
     size_t few_parts = 0, chunk_parts = 0;                         // rows of partial results
 };
 
-Plan plan_of(const nnz_paged_kv &kv, const nnz_paged_batch &b, uint32_t hq) {
+// window: where no row's keys are more than that, else 0.  A few rows (16 tokens)
+// then see window + 15 keys, of them up to 31 more for whole steps of 32; a row
+// tile (128 tokens) window + 127, up to 63 more for whole tiles.
+Plan plan_of(const nnz_paged_kv &kv, const nnz_paged_batch &b, uint32_t hq, uint32_t window = 0) {
     Plan p;
+    auto keys = [&](uint32_t more) {
+        return window ? (uint32_t)std::min<uint64_t>(b.max_kv_len, (uint64_t)window + more) : b.max_kv_len;
+    };
     const uint32_t G = hq / kv.num_kv_heads, hkv = kv.num_kv_heads;
     const uint64_t most = (uint64_t)b.max_q_len * G;   // rows of a sequence
     const bool chunks = most > FEW;
     // One sequence whose bound passes 16 rows goes to chunk_part, whatever its
     // length turns out to be; a batch of several may hold both kinds.
     if (G <= FEW && (!chunks || b.num_seqs > 1)) {
-        const uint32_t steps = (b.max_kv_len + 31) / 32, blocks = b.num_seqs * hkv;   // below 2^26
+        const uint32_t steps = (keys(48) + 31) / 32, blocks = b.num_seqs * hkv;   // below 2^26
         const uint32_t want = std::max(1u, (chunks ? 256u : 1024u) / blocks), most_splits = std::max(1u, steps / 16);
         const uint32_t splits = std::min({want, most_splits, MOST_SPLITS});
         p.few_rows = (uint32_t)std::min<uint64_t>(most, FEW);
@@ -930,7 +936,7 @@ Plan plan_of(const nnz_paged_kv &kv, const nnz_paged_batch &b, uint32_t hq) {
         const uint64_t by_rows = (uint64_t)b.num_rows * G / TILE_ROWS + b.num_seqs;
         const uint64_t by_seqs = (uint64_t)b.num_seqs * ((most + TILE_ROWS - 1) / TILE_ROWS);
         p.units = (uint32_t)std::min(by_rows, by_seqs);
-        const uint32_t tiles = (b.max_kv_len + KT - 1) / KT;
+        const uint32_t tiles = (keys(192) + KT - 1) / KT;
         const uint32_t blocks = kv.head_dim == 64 || b.num_seqs > 1 ? 512 : 256;
         const uint32_t want = (uint32_t)std::max<uint64_t>(1, blocks / ((uint64_t)p.units * hkv)), most_splits = std::max(1u, tiles / 4);
         const uint32_t splits = std::min({want, most_splits, MOST_SPLITS});
@@ -1001,8 +1007,12 @@ extern "C" int nnz_dispatch_paged_attention(nnz_ctx *ctx, const nnz_paged_kv *kv
     NNZ_CHECK_CTX(ctx);
     if (const PagedFault f = paged_attn_fault(kv, batch, q, output, lse, p); f.code)
         return nnz_fail(ctx, f.code, "paged_attention: %s", f.what);
-    const Plan plan = plan_of(*kv, *batch, p->num_query_heads);
+    Plan plan = plan_of(*kv, *batch, p->num_query_heads);
     const size_t need = bytes_of(plan, kv->head_dim);
+    if (p->window && !p->prefix_lens) {   // fewer keys to split, in the workspace that the bounds ask for
+        const Plan narrow = plan_of(*kv, *batch, p->num_query_heads, p->window);
+        if (bytes_of(narrow, kv->head_dim) <= need) plan = narrow;
+    }
     NNZ_REQUIRE(ctx, blocks_of(plan, *batch, kv->num_kv_heads) < (1u << 23), NNZ_EUNSUPPORTED,
                 "paged_attention: more than 2^23 blocks; split the batch");
     NNZ_REQUIRE(ctx, need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0), NNZ_EINVAL,

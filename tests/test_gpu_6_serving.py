@@ -400,6 +400,20 @@ def test_long_context_splits(dev):
         _check_attention(c, kp, vp, q, out, lse, rows=4, **o)
 
 
+@pytest.mark.parametrize("d,hq,hkv,n,lens", [
+    (64, 2, 2, [1], [6001]), (128, 4, 4, [16], [5999]), (128, 2, 2, [300], [6050]), (64, 4, 2, [129], [6127]),
+    (64, 2, 2, [1, 200, 16], [6100, 3333, 6031])])
+def test_windows_wherever_they_begin(dev, d, hq, hkv, n, lens):
+    """Keys are split by what a window can show; rows whose keys begin and end
+    anywhere in the steps and tiles of that see all of them."""
+    for shift, window in enumerate((1, 481, 512, 513, 1023, 2000, 2017, 5000, 2**32 - 1)):
+        c = R.Case(n, [x - 13 * shift for x in lens], hq, hkv, d, 32, F16, seed=shift)
+        q = c.normal(c.T, hq, d)
+        kp, vp = c.normal(c.total, hkv, 32, d), c.normal(c.total, hkv, d, 32)
+        out, lse = _attention(dev, c, kp, vp, q, window=window)
+        _check_attention(c, kp, vp, q, out, lse, rows=6, window=window)
+
+
 def test_attention_agrees_with_the_contiguous_operator(dev):
     """A decode step over pages equals nnz_dispatch_gqa_attention on the same
     tokens in one contiguous cache, to the rounding of weights and store."""
