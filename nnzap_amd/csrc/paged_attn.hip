@@ -21,7 +21,7 @@
 //
 // Measured (kernels' time): one token over 131072 (32 + 8 heads of 128, bf16, 537
 // MB) 95 + 8 us, 5.6 TB/s; 64 chats of up to 8191 (1.17 GB) 238 + 5, 4.9 TB/s; 2048
-// tokens over 8192 (16 + 8 heads of 128, 155 GFLOP) 171 us, 0.9 PFLOP/s: there 256
+// tokens over 8192 (16 + 8 heads of 128, 155 GFLOP) 165-172 us, 0.9 PFLOP/s: there 256
 // KB of LDS reads a turn take 3000 of a CU's 4400 cycles, vector instructions 2600,
 // the matrix cores 2048; 64 rows a wave would halve the reads, but leave one wave
 // a SIMD.
