@@ -641,6 +641,8 @@ class PagedBatch:
         seqs, width = page_table.shape
         _refuse(q_starts.shape != (seqs + 1,) or kv_lens.shape != (seqs,), n,
                 "q_starts is [num_seqs + 1], kv_lens [num_seqs]")
+        _refuse(not all(0 < x < 1 << 32 for x in (num_rows, max_q_len, max_kv_len)), n,
+                "num_rows, max_q_len and max_kv_len are positive")
         self.page_table, self.q_starts, self.kv_lens = page_table, q_starts, kv_lens
         self.num_rows, self.num_seqs, self.device = num_rows, seqs, page_table.device
         self.desc = L.PagedBatchDesc(page_table.data_ptr(), q_starts.data_ptr(),
@@ -684,7 +686,7 @@ def dispatch_paged_attention(dev, kv: PagedKVCache, batch: PagedBatch, q, out, w
     n, rows, at = "nnz_dispatch_paged_attention", batch.num_rows, kv.device
     hq = q.shape[1] if q.dim() == 3 else 0
     _refuse(batch.device != at, n, "batch and cache are on two devices")
-    _refuse(window < 0, n, "window must not be negative")
+    _refuse(not 0 <= window < 1 << 32, n, "window is 0 (none) to 2^32 - 1")
     p = L.PagedAttnParams(_flat(slopes, (hq,), _T.f32, at, n, "slopes"),
                           _flat(prefix_lens, (batch.num_seqs,), _T.i32, at, n, "prefix_lens"), hq,
                           _rows_of(kv, q, rows, hq, n, "q"), _rows_of(kv, out, rows, hq, n, "out"),

@@ -268,6 +268,9 @@ def test_batch_tensors_are_checked():
                 (t.t().contiguous().t(), s, ln)):
         with pytest.raises(NnzError):
             ops.PagedBatch(*bad, 6, 3, 40)
+    for bad in ((0, 3, 40), (6, -3, 40), (6, 3, 2**32 + 40)):
+        with pytest.raises(NnzError):
+            ops.PagedBatch(t, s, ln, *bad)
 
 
 def test_rows_of_another_shape_or_type_are_refused():
@@ -282,7 +285,8 @@ def test_rows_of_another_shape_or_type_are_refused():
         with pytest.raises(NnzError):
             ops.dispatch_paged_append(CPU, c, b, **a)
     for bad in (dict(q=q[:, :, :32]), dict(out=q[:3]), dict(lse=torch.zeros(4, 6)), dict(slopes=torch.zeros(2)),
-                dict(window=-1), dict(prefix_lens=torch.zeros(2)), dict(prefix_lens=torch.zeros(3, dtype=torch.int32))):
+                dict(window=-1), dict(window=2**32 + 1),
+                dict(prefix_lens=torch.zeros(2)), dict(prefix_lens=torch.zeros(3, dtype=torch.int32))):
         a = {**dict(q=q, out=q.clone(), workspace=None), **bad}
         with pytest.raises(NnzError):
             ops.dispatch_paged_attention(CPU, c, b, **a)
